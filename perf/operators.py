@@ -1,0 +1,431 @@
+"""What the rows operators compute, and the sizes at which they are measured.
+
+The rows operators (include/speech_hip.h, speech_rows_*) work on frame-major matrices on the device: a batch's features, or
+what a model's first layers make of them, one row per frame.
+
+  drop      Y = keep X / (1 - p); the mask comes from a counter-based generator keyed by (seed, the row's key, column) and is
+            never stored, so the same call on the gradient is the backward pass
+  norm      H = R + keep X / (1 - p) rounded to the data's type, rstd = 1 / sqrt(mean(H^2) + eps), Y = H rstd weight; or Y in
+            8 bits: e4m3 values Q with one power-of-two scale S (its biased exponent, e8m0) per block of 128 columns
+  grad      the gradients of norm: of the residual stream, of the dropped input and of the weight
+  project   X quantized in blocks of 128, times a weight matrix held in the same form, plus a bias
+  product   the same product of two matrices that are held in 8 bits already
+  chain     norm with its 8-bit output, and the product that reads it
+  project_grad   both gradients of project, from the output's gradient: dX = q(dY) q(W^T)^T, dW = q(dY^T) q(X^T)^T
+
+own = False computes them in plain torch operations, own = True calls the framework.
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+BLOCK = 128                 # columns that share a scale
+E4M3_MAX = 448.0
+EPS = 1e-6
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+M64 = (1 << 64) - 1
+
+
+def listed():
+    return [
+        # one second of 80-bin log-mel features with feature dropout: what a streaming or test-sized call costs
+        dict(name="drop fbank 1 s", op="drop", rows=98, cols=80, type="f32", p=0.1),
+        # 30 utterances of 10 s, spectrogram rows: 257 columns, no row but the first starts on 16 bytes
+        dict(name="drop spectrogram", op="drop", rows=29940, cols=257, type="f32", p=0.2),
+        # hidden activations of a training batch: 128 utterances of 10 s
+        dict(name="drop hidden", op="drop", rows=127744, cols=1024, type="bf16", p=0.1),
+        # one new frame at a time, before an 8-bit product
+        dict(name="norm one frame 8-bit", op="norm", rows=1, cols=2048, type="bf16", out="e4m3", residual=True, p=0.0),
+        # a serving batch: 8 utterances of 10 s, residual stream in and out, 8-bit output
+        dict(name="norm serving 8-bit", op="norm", rows=7984, cols=1024, type="bf16", out="e4m3", residual=True, p=0.0),
+        # a training batch: 32 utterances of 10 s, residual + dropped branch, 16-bit output and the row statistics
+        dict(name="norm training", op="norm", rows=31936, cols=1024, type="bf16", out="same", residual=True, p=0.1),
+        # the same batch's backward pass
+        dict(name="grad training", op="grad", rows=31936, cols=1024, type="bf16", residual=True, p=0.1),
+        # backward on one utterance's spectrogram rows in 32 bits, rows of 257
+        dict(name="grad spectrogram", op="grad", rows=998, cols=257, type="f32", residual=False, p=0.0),
+        # one new frame through norm and product: reads the weights, 8 MiB, once
+        dict(name="chain one frame", op="chain", rows=1, n=4096, k=2048, type="bf16", bias=False),
+        # a 10 s utterance, 9 spliced 80-bin frames a row, into the first layer: K is no multiple of 128
+        dict(name="project spliced fbank", op="project", rows=998, n=512, k=720, type="f16", bias=True),
+        # the training batch's wide layer
+        dict(name="product wide", op="product", rows=31936, n=4096, k=2048, type="bf16", bias=False),
+        # gradients of a layer, activations and weights quantized along the other axis
+        dict(name="project_grad layer", op="project_grad", rows=7984, n=2048, k=1024, type="bf16"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["drop", "norm", "norm", "grad", "chain", "project", "product", "project_grad"])
+    kind = rng.choice(["f32", "bf16", "bf16", "f16"])
+    if op in ("drop", "norm", "grad"):
+        cols = _log(rng, 13, 4096)
+        rows = _log(rng, 1, min(127744, 32000000 // cols))
+        c = dict(op=op, rows=rows, cols=cols, type=kind, p=rng.choice([0.0, 0.05, 0.1, 0.2, 0.5]))
+        if op == "drop":
+            c["p"] = c["p"] or 0.3
+        else:
+            c["residual"] = rng.random() < 0.7
+        if op == "norm":
+            c["out"] = rng.choice(["same", "e4m3"])
+        return c
+    n, k = _log(rng, 16, 4096), _log(rng, 24, 4096)
+    rows = _log(rng, 1, min(31936, 60000000000 // (n * k)))
+    c = dict(op=op, rows=rows, n=n, k=k, type=kind)
+    if op != "project_grad":
+        c["bias"] = rng.random() < 0.5
+    return c
+
+
+# ---- inputs ----
+
+def _pad(n, to):
+    return -(-n // to) * to
+
+
+def _activations(g, rows, cols, dtype):
+    """what a normalised feature matrix or a residual stream looks like: unit normal, some wide columns, some silent (zero) rows"""
+    x = torch.randn(rows, cols, generator=g, device="cuda")
+    x *= torch.where(torch.rand(cols, generator=g, device="cuda") < 0.02, 12.0, 1.0)
+    if rows > 4:
+        x *= (torch.rand(rows, 1, generator=g, device="cuda") >= 0.01).float()
+    return x.to(dtype)
+
+
+def _held(rows, cols):
+    """room for a matrix in 8 bits: e4m3 values, rows padded to 16 bytes, and its block exponents, rows padded to 4"""
+    q = torch.zeros(rows, _pad(cols, 16), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[:, :cols]
+    s = torch.zeros(rows, _pad(-(-cols // BLOCK), 4), dtype=torch.uint8, device="cuda")[:, :-(-cols // BLOCK)]
+    return q, s
+
+
+def _hold(x, q, s):
+    v, e = _quantize(x)
+    q.copy_(v)
+    s.copy_(e)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed * 7919 + 17)
+    dtype = TYPES[case["type"]]
+    st = dict(case)
+    st["seed"] = (0x9E3779B97F4A7C15 * (seed + 1)) & M64
+    rows = case["rows"]
+    # rows are frames of utterances of 998: the key of a row is its utterance's number and its frame's
+    r = torch.arange(rows, device="cuda", dtype=torch.int64)
+    st["keys"] = ((r // 998 + 5) << 32) | (r % 998)
+    if case["op"] in ("drop", "norm", "grad"):
+        cols = case["cols"]
+        st["X"] = _activations(g, rows, cols, dtype)
+        new = lambda: torch.empty(rows, cols, dtype=dtype, device="cuda")  # noqa: E731
+        if case["op"] == "drop":
+            st["Y"] = new()
+            return st
+        st["weight"] = (1.0 + 0.1 * torch.randn(cols, generator=g, device="cuda")).to(dtype)
+        st["R"] = _activations(g, rows, cols, dtype) if case["residual"] else None
+        st["rstd"] = torch.empty(rows, dtype=torch.float32, device="cuda")
+        if case["op"] == "norm":
+            st["H"] = new()
+            st["Y"] = new() if case["out"] == "same" else None
+            st["Q"], st["S"] = _held(rows, cols) if case["out"] == "e4m3" else (None, None)
+            return st
+        # what the forward pass left, and the gradients that arrive
+        h = st["X"].float() if st["R"] is None else (st["R"].float() + st["X"].float())
+        st["H"] = h.to(dtype)
+        st["rstd"] = torch.rsqrt(st["H"].double().square().mean(1) + EPS).float()
+        st["dY"] = (0.02 * torch.randn(rows, cols, generator=g, device="cuda")).to(dtype)
+        st["dR"] = (0.02 * torch.randn(rows, cols, generator=g, device="cuda")).to(dtype) if case["residual"] else None
+        del st["X"], st["R"]
+        st["dH"] = new()
+        st["dX"] = new() if case["p"] > 0 else None
+        st["dW"] = torch.empty(cols, dtype=torch.float32, device="cuda")
+        st["work"] = torch.empty(4 * 1024 * cols + 256, dtype=torch.uint8, device="cuda")
+        return st
+    n, k = case["n"], case["k"]
+    X = _activations(g, rows, k, dtype)
+    W = torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k)
+    if case["op"] == "project_grad":
+        st["X"] = X
+        st["dY"] = (0.02 * torch.randn(rows, n, generator=g, device="cuda")).to(dtype)
+        st["Wt"], st["SWt"] = _held(k, n)                  # the weights, laid out once along the axis that dX sums over
+        _hold(W.t().contiguous(), st["Wt"], st["SWt"])
+        st["Qy"], st["Sy"] = _held(rows, n)
+        st["Qyt"], st["Syt"] = _held(n, rows)
+        st["Qxt"], st["Sxt"] = _held(k, rows)
+        st["dX"] = torch.empty(rows, k, dtype=dtype, device="cuda")
+        st["dW"] = torch.empty(n, k, dtype=torch.float32, device="cuda")
+        return st
+    st["W"], st["SW"] = _held(n, k)
+    _hold(W, st["W"], st["SW"])
+    st["b"] = 0.1 * torch.randn(n, generator=g, device="cuda") if case["bias"] else None
+    st["Q"], st["S"] = _held(rows, k)
+    st["Y"] = torch.empty(rows, n, dtype=dtype, device="cuda")
+    if case["op"] == "product":
+        _hold(X, st["Q"], st["S"])
+        return st
+    st["X"] = X
+    if case["op"] == "chain":
+        st["weight"] = (1.0 + 0.1 * torch.randn(k, generator=g, device="cuda")).to(dtype)
+        st["R"] = _activations(g, rows, k, dtype)
+        st["H"] = torch.empty_like(X)
+    return st
+
+
+# ---- plain forms ----
+
+def _shr(z, n):
+    return (z >> n) & ((1 << (64 - n)) - 1)
+
+
+def _signed(v):
+    v &= M64
+    return v - (1 << 64) if v >> 63 else v
+
+
+def _mix64(z):
+    z = z + _signed(0x9E3779B97F4A7C15)
+    z = (z ^ _shr(z, 30)) * _signed(0xBF58476D1CE4E5B9)
+    z = (z ^ _shr(z, 27)) * _signed(0x94D049BB133111EB)
+    return z ^ _shr(z, 31)
+
+
+def _kept(seed, keys, cols, p):
+    """the mask: 32 random bits for each (row, column), kept where they are at least p 2^32"""
+    ku = _mix64(torch.full((1,), _signed(seed ^ 0xD1B54A32D192ED03), dtype=torch.int64, device=keys.device))
+    fk = _mix64(ku ^ keys)
+    i = (torch.arange(cols, device=keys.device, dtype=torch.int64) * 0x9E3779B9) & 0xFFFFFFFF
+    h = (fk & 0xFFFFFFFF)[:, None] ^ i[None, :]
+    h = ((h ^ (h >> 16)) * 0x85EBCA6B) & 0xFFFFFFFF
+    h = ((h ^ (h >> 13)) * 0xC2B2AE35) & 0xFFFFFFFF
+    h = ((h ^ (h >> 16)) + _shr(fk, 32)[:, None]) & 0xFFFFFFFF
+    return h >= int(p * 4294967296.0)
+
+
+def _dropped(st, x):
+    if st["p"] == 0.0:
+        return x.float()
+    return torch.where(_kept(st["seed"], st["keys"], x.shape[1], st["p"]), x.float() * (1.0 / (1.0 - st["p"])), 0.0)
+
+
+def _quantize(x):
+    """(e4m3 values, biased exponents): each block of 128 columns is divided by the smallest power of two that brings its
+    largest value to at most 448; a block of zeros takes the smallest scale, 2^-127"""
+    rows, cols = x.shape
+    nb = -(-cols // BLOCK)
+    v = torch.nn.functional.pad(x.float(), (0, nb * BLOCK - cols)).view(rows, nb, BLOCK)
+    m, e = torch.frexp(v.abs().amax(2))                        # amax = m 2^e, m in [0.5, 1): at most 448 = 0.875 2^9 times 2^(e - 9)
+    e = torch.where(m > 0.875, e - 8, e - 9).clamp(min=-127)
+    e = torch.where(m == 0, -127, e)
+    q = torch.ldexp(torch.ldexp(v, (-(e // 2))[:, :, None]), (-(e - e // 2))[:, :, None])
+    return q.view(rows, nb * BLOCK)[:, :cols].to(torch.float8_e4m3fn), (e + 127).to(torch.uint8)
+
+
+def _stands_for(q, s, dtype=torch.float32):
+    """the values that a matrix in 8 bits stands for"""
+    e = (s.to(torch.int32) - 127).repeat_interleave(BLOCK, dim=1)[:, :q.shape[1]]
+    return torch.ldexp(q.to(dtype), e)
+
+
+def _norm(st):
+    x = _dropped(st, st["X"]) if "p" in st else st["X"].float()
+    h = (x if st["R"] is None else st["R"].float() + x).to(st["X"].dtype)
+    rstd = torch.rsqrt(h.float().square().mean(1) + EPS)
+    return h, rstd, h.float() * rstd[:, None] * st["weight"].float()
+
+
+def _times(a, sa, b, sb, bias, dtype):
+    y = _stands_for(a, sa) @ _stands_for(b, sb).t()
+    return (y if bias is None else y + bias).to(dtype)
+
+
+def _plain(st):
+    op = st["op"]
+    if op == "drop":
+        return _dropped(st, st["X"]).to(st["X"].dtype)
+    if op == "norm":
+        h, rstd, y = _norm(st)
+        if st["out"] == "same":
+            return {"H": h, "Y": y.to(h.dtype), "rstd": rstd}
+        q, s = _quantize(y)
+        return {"H": h, "Q": q, "S": s.view(torch.float8_e8m0fnu)}
+    if op == "grad":
+        h, rstd = st["H"].float(), st["rstd"][:, None]
+        dy = st["dY"].float()
+        wdy = dy * st["weight"].float()
+        dh = rstd * wdy - h * rstd.pow(3) * (wdy * h).mean(1, keepdim=True)
+        if st["dR"] is not None:
+            dh = dh + st["dR"].float()
+        out = {"dH": dh.to(st["H"].dtype), "dW": (dy * h * rstd).sum(0)}
+        if st["dX"] is not None:
+            out["dX"] = _dropped(st, dh).to(st["H"].dtype)
+        return out
+    if op == "project_grad":
+        q, s = _quantize(st["dY"])
+        qt, t = _quantize(st["dY"].t())
+        xt, u = _quantize(st["X"].t())
+        return {"dX": _times(q, s, st["Wt"], st["SWt"], None, st["X"].dtype), "dW": _times(qt, t, xt, u, None, torch.float32)}
+    if op == "product":
+        return _times(st["Q"], st["S"], st["W"], st["SW"], st["b"], st["Y"].dtype)
+    if op == "project":
+        q, s = _quantize(st["X"])
+        return _times(q, s, st["W"], st["SW"], st["b"], st["Y"].dtype)
+    h, _, y = _norm(st)
+    q, s = _quantize(y)
+    return {"H": h, "Y": _times(q, s, st["W"], st["SW"], st["b"], st["Y"].dtype)}
+
+
+# ---- the framework's calls ----
+
+def _own(st):
+    from speech_amd import api
+    op = st["op"]
+    if op == "drop":
+        api.dropout(st["X"], st["Y"], st["p"], st["seed"], keys=st["keys"])
+        return st["Y"]
+    if op == "norm":
+        api.rms_norm(st["X"], st["weight"], EPS, residual=st["R"], H=st["H"], Y=st["Y"], Q=st["Q"], S=st["S"],
+                     rstd=st["rstd"] if st["Y"] is not None else None, p=st["p"], seed=st["seed"], keys=st["keys"])
+        if st["Y"] is not None:
+            return {"H": st["H"], "Y": st["Y"], "rstd": st["rstd"]}
+        return {"H": st["H"], "Q": st["Q"], "S": st["S"].view(torch.float8_e8m0fnu)}
+    if op == "grad":
+        api.rms_norm_backward(st["dY"], st["H"], st["weight"], st["rstd"], st["dH"], dR=st["dR"], dX=st["dX"], dW=st["dW"], work=st["work"],
+                              p=st["p"], seed=st["seed"], keys=st["keys"])
+        out = {"dH": st["dH"], "dW": st["dW"]}
+        if st["dX"] is not None:
+            out["dX"] = st["dX"]
+        return out
+    if op == "project_grad":
+        api.quantize(st["dY"], st["Qy"], st["Sy"])
+        api.quantize(st["dY"], st["Qyt"], st["Syt"], transpose=True)
+        api.quantize(st["X"], st["Qxt"], st["Sxt"], transpose=True)
+        api.product(st["Qy"], st["Sy"], st["Wt"], st["SWt"], st["dX"])
+        api.product(st["Qyt"], st["Syt"], st["Qxt"], st["Sxt"], st["dW"])
+        return {"dX": st["dX"], "dW": st["dW"]}
+    if op == "project":
+        api.quantize(st["X"], st["Q"], st["S"])
+    elif op == "chain":
+        api.rms_norm(st["X"], st["weight"], EPS, residual=st["R"], H=st["H"], Q=st["Q"], S=st["S"])
+    api.product(st["Q"], st["S"], st["W"], st["SW"], st["Y"], bias=st["b"])
+    return {"H": st["H"], "Y": st["Y"]} if op == "chain" else st["Y"]
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return _plain(state)
+
+
+# ---- bounds and exact values ----
+
+def work(case):
+    b = {"f32": 4, "bf16": 2, "f16": 2}[case["type"]]
+    rows = case["rows"]
+    if case["op"] in ("drop", "norm", "grad"):
+        n = rows * case["cols"]
+        key = 8 * rows if case["p"] > 0 else 0
+        if case["op"] == "drop":
+            return {"bytes": 2 * b * n + key, "flops": n}
+        if case["op"] == "norm":
+            out = b * n + 4 * rows if case["out"] == "same" else n + rows * -(-case["cols"] // BLOCK)
+            return {"bytes": (3 if case["residual"] else 2) * b * n + out + key, "flops": 6 * n}
+        moved = 3 + (1 if case["residual"] else 0) + (1 if case["p"] > 0 else 0)
+        return {"bytes": moved * b * n + key + 4 * rows, "flops": 12 * n}
+    n, k = case["n"], case["k"]
+    weights, held = n * k + n * -(-k // BLOCK), rows * k + rows * -(-k // BLOCK)
+    if case["op"] == "project_grad":
+        return {"bytes": b * rows * (n + k) + weights + b * rows * k + 4 * n * k, "flops": 4.0 * rows * n * k}
+    y = b * rows * n
+    x = {"product": held, "project": b * rows * k, "chain": 3 * b * rows * k}[case["op"]]
+    return {"bytes": x + weights + y, "flops": 2.0 * rows * n * k}
+
+
+def _exact_mask(seed, keys, cols, p):
+    """the mask once more, in unsigned numpy arithmetic"""
+    def mix(z):
+        z = z + np.uint64(0x9E3779B97F4A7C15)
+        z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+        z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+        return z ^ (z >> np.uint64(31))
+    with np.errstate(over="ignore"):
+        ku = mix(np.full(1, seed ^ 0xD1B54A32D192ED03, dtype=np.uint64))
+        fk = mix(ku ^ keys.cpu().numpy().astype(np.uint64))
+        h = (fk & np.uint64(0xFFFFFFFF)).astype(np.uint32)[:, None] ^ (np.arange(cols, dtype=np.uint32) * np.uint32(0x9E3779B9))[None, :]
+        h ^= h >> np.uint32(16)
+        h *= np.uint32(0x85EBCA6B)
+        h ^= h >> np.uint32(13)
+        h *= np.uint32(0xC2B2AE35)
+        h ^= h >> np.uint32(16)
+        h += (fk >> np.uint64(32)).astype(np.uint32)[:, None]
+    return torch.from_numpy(h >= np.uint32(int(p * 2.0 ** 32))).cuda()
+
+
+def _exact_held(x):
+    """(values as e4m3 would hold them but for its rounding, exponents) in 64 bits"""
+    rows, cols = x.shape
+    nb = -(-cols // BLOCK)
+    v = torch.zeros(rows, nb * BLOCK, dtype=torch.float64, device="cuda")
+    v[:, :cols] = x
+    top = v.view(rows, nb, BLOCK).abs().amax(2)
+    e = torch.ceil(torch.log2(top / E4M3_MAX)).clamp(-127, 127)
+    e = torch.where(top > E4M3_MAX * torch.exp2(e), e + 1, torch.where((top <= E4M3_MAX * torch.exp2(e - 1)) & (e > -127), e - 1, e))
+    return (v.view(rows, nb, BLOCK) * torch.exp2(-e)[:, :, None]).view(rows, -1)[:, :cols], torch.exp2(e)
+
+
+def _exact_rounded(x):
+    """what x stands for once it is held in 8 bits, in 64 bits: 4 significant bits, steps of 2^-9 below 2^-6"""
+    v, scale = _exact_held(x)
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    return torch.round(v / step) * step * scale.repeat_interleave(BLOCK, dim=1)[:, :x.shape[1]]
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    op = case["op"]
+    X = st["X"].double() if "X" in st else None
+    p = case.get("p", 0.0)
+    if op in ("drop", "norm", "grad"):
+        mask = _exact_mask(st["seed"], st["keys"], case["cols"], p) if p > 0 else None
+        drop = (lambda v: v) if mask is None else (lambda v: torch.where(mask, v / (1.0 - p), torch.zeros((), dtype=torch.float64, device="cuda")))
+    if op == "drop":
+        return drop(X)
+    if op in ("norm", "chain"):
+        x = drop(X) if op == "norm" else X
+        h = x if st["R"] is None else x + st["R"].double()
+        hr = h.to(st["X"].dtype).double()
+        rstd = 1.0 / torch.sqrt((hr * hr).mean(1) + EPS)
+        y = hr * rstd[:, None] * st["weight"].double()
+        if op == "chain":
+            w = _stands_for(st["W"], st["SW"], torch.float64)
+            out = _exact_rounded(y) @ w.t()
+            return {"H": h, "Y": out if st["b"] is None else out + st["b"].double()}
+        if case["out"] == "same":
+            return {"H": h, "Y": y, "rstd": rstd}
+        q, s = _exact_held(y)
+        return {"H": h, "Q": q, "S": s}
+    if op == "grad":
+        h, r, dy, w = st["H"].double(), st["rstd"].double()[:, None], st["dY"].double(), st["weight"].double()
+        g = dy * w
+        dh = r * (g - h * r * r * (g * h).sum(1, keepdim=True) / case["cols"])
+        if st["dR"] is not None:
+            dh = dh + st["dR"].double()
+        out = {"dH": dh, "dW": (dy * h * r).sum(0)}
+        if p > 0:
+            out["dX"] = drop(dh)
+        return out
+    if op == "project_grad":
+        dy = st["dY"].double()
+        wt = _stands_for(st["Wt"], st["SWt"], torch.float64)
+        return {"dX": _exact_rounded(dy) @ wt.t(), "dW": _exact_rounded(dy.t().contiguous()) @ _exact_rounded(X.t().contiguous()).t()}
+    w = _stands_for(st["W"], st["SW"], torch.float64)
+    a = _stands_for(st["Q"], st["S"], torch.float64) if op == "product" else _exact_rounded(X)
+    y = a @ w.t()
+    return y if st["b"] is None else y + st["b"].double()
