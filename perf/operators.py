@@ -76,6 +76,7 @@ def draw(rng):
         if op == "norm":
             c["out"] = rng.choice(["same", "e4m3"])
         return c
+    kind = rng.choice(["bf16", "f16"])                     # the product's outputs have 16 bits
     n, k = _log(rng, 16, 4096), _log(rng, 24, 4096)
     rows = _log(rng, 1, min(31936, 60000000000 // (n * k)))
     c = dict(op=op, rows=rows, n=n, k=k, type=kind)
@@ -161,7 +162,7 @@ def prepare(case, seed):
         st["Qyt"], st["Syt"] = _held(n, rows)
         st["Qxt"], st["Sxt"] = _held(k, rows)
         st["dX"] = torch.empty(rows, k, dtype=dtype, device="cuda")
-        st["dW"] = torch.empty(n, k, dtype=torch.float32, device="cuda")
+        st["dW"] = torch.empty(n, k, dtype=dtype, device="cuda")
         return st
     st["W"], st["SW"] = _held(n, k)
     _hold(W, st["W"], st["SW"])
@@ -271,7 +272,7 @@ def _plain(st):
         q, s = _quantize(st["dY"])
         qt, t = _quantize(st["dY"].t())
         xt, u = _quantize(st["X"].t())
-        return {"dX": _times(q, s, st["Wt"], st["SWt"], None, st["X"].dtype), "dW": _times(qt, t, xt, u, None, torch.float32)}
+        return {"dX": _times(q, s, st["Wt"], st["SWt"], None, st["X"].dtype), "dW": _times(qt, t, xt, u, None, st["X"].dtype)}
     if op == "product":
         return _times(st["Q"], st["S"], st["W"], st["SW"], st["b"], st["Y"].dtype)
     if op == "project":
@@ -342,7 +343,7 @@ def work(case):
     n, k = case["n"], case["k"]
     weights, held = n * k + n * -(-k // BLOCK), rows * k + rows * -(-k // BLOCK)
     if case["op"] == "project_grad":
-        return {"bytes": b * rows * (n + k) + weights + b * rows * k + 4 * n * k, "flops": 4.0 * rows * n * k}
+        return {"bytes": b * rows * (n + k) + weights + b * rows * k + b * n * k, "flops": 4.0 * rows * n * k}
     y = b * rows * n
     x = {"product": held, "project": b * rows * k, "chain": 3 * b * rows * k}[case["op"]]
     return {"bytes": x + weights + y, "flops": 2.0 * rows * n * k}
