@@ -19,7 +19,7 @@ extern "C" {
 #endif
 
 enum { SPEECH_SPECTROGRAM = 0, SPEECH_FBANK = 1, SPEECH_MFCC = 2, SPEECH_PLP = 3 };
-enum { SPEECH_F32 = 0, SPEECH_F64 = 1 };
+enum { SPEECH_F32 = 0, SPEECH_F64 = 1, SPEECH_BF16 = 2, SPEECH_F16 = 3 };   /* the 16-bit types: rows operators only */
 
 /* The union of the reference functions' option lists (c/codee_speech.h:13-25). */
 typedef struct speech_opts {
@@ -186,6 +186,116 @@ void speech_set_dropin_dither(unsigned long long seed, long long utt);
 int speech_batch_synth_audio(speech_batch *batch, void *X_dev, int pcm16, unsigned long long seed, const unsigned long long *ids, void *stream);
 /* The same generator on the host (no device needed): samples 0 .. n-1 of corpus utterance `utt` as int16. */
 int speech_synth_audio_host(unsigned long long seed, unsigned long long utt, size_t n, short *out);
+
+/* ---- rows operators: a batch's packed frames on their way into a model (no counterpart in the reference) ----
+   They work on frame-major matrices in device memory: `rows` rows of `cols` elements, row i at X + i * ldx elements, ldx >=
+   cols; nothing behind column cols and nothing behind the last row is written.  The matrices of a densely packed batch
+   (speech_batch_run, _add_deltas, _splice: total_frames rows) and of splice_subsample (total_rows rows) are such matrices.
+   `device` is the HIP device that holds every pointer and owns the stream.  All enqueue on `stream` and return; none
+   allocates, synchronises or keeps anything between calls, so all can be captured into a graph.  rows == 0 does nothing
+   (but that a dW asked for becomes 0).
+   Sums are kept in 32-bit floats, the result does not depend on scheduling: the same call gives the same bits.  Unless said
+   otherwise an output must not overlap another argument; an output that may be an input of the same call is that input, with
+   the same row stride, and not a part of it.
+   dtype: SPEECH_F32, SPEECH_BF16 or SPEECH_F16, and for dropout SPEECH_F64 too. */
+
+/* Dropout without a stored mask: element (i, j) is kept when 32 random bits, a counter-based hash of (seed + *step, keys[i], j),
+   are at least floor(p 2^32); what is kept is multiplied by 1 / (1 - p), what is dropped is +0 whatever it held.  The same
+   arguments draw the same mask: the backward pass is the same call on the gradient.
+     p     probability of dropping, 0 <= p < 1 (0 keeps everything and draws nothing)
+     seed  one for each layer and training step
+     step  NULL, or a number on the device that is added to the seed when the kernel runs: a captured graph that also advances
+           the number draws another mask on every replay
+     keys  NULL: row i has the key i; or a key for each row on the device.  speech_batch_row_keys makes them of the
+           utterances' numbers and frames, so that batches and shards of a corpus draw the masks that one batch would */
+typedef struct speech_drop {
+    double p;
+    unsigned long long seed;
+    const unsigned long long *step;
+    const unsigned long long *keys;
+} speech_drop;
+
+/* Keys of a batch's rows, as splice_subsample packs them (n = 1, offset = 0: every frame, the packing of a dense batch): the row
+   of frame w of utterance u gets id << 32 | w, id being u or what speech_batch_set_ids gave.  keys_dev holds the total of
+   speech_batch_subsample_rows(n, offset) keys.  The batch's first call allocates a number for each utterance, which its calls share:
+   calls on one batch that overlap on the device race. */
+int speech_batch_row_keys(speech_batch *batch, int n, int offset, unsigned long long *keys_dev, void *stream);
+
+/* Y = dropout of X.  Y may be X. */
+int speech_rows_dropout(int device, int dtype, size_t rows, size_t cols, const void *X, size_t ldx, void *Y, size_t ldy,
+                        const speech_drop *drop, void *stream);
+
+/* Root-mean-square norm of rows, with the residual stream's addition in front and 8-bit output behind:
+     h = R + dropout(X), rounded to dtype;  rstd = 1 / sqrt(mean of h^2 over the row + eps);  y = h rstd weight
+   R       NULL: no residual.            drop    NULL or p = 0: no dropout.
+   H       NULL, or gets h (the next residual stream, and what the backward pass reads).  May be X or R.
+   Y       NULL, or gets y rounded to dtype.  May be X or R, unless H is that one.
+   Q, S    NULL, or get y held in 8 bits in the form of speech_rows_quantize, rounded once from 32 bits.  At least one of Y
+           and Q is given.
+   rstd    NULL, or rows floats for the backward pass.
+   weight  NULL (ones) or cols factors, of dtype or, with weight_f32 != 0, floats.
+   eps     positive.
+   A row whose sum of squares passes the range of a float has rstd 0; NaN and infinities stay in their row. */
+typedef struct speech_norm {
+    int dtype, weight_f32;
+    size_t rows, cols;
+    double eps;
+    const void *X; size_t ldx;
+    const void *R; size_t ldr;
+    const void *weight;
+    void *H; size_t ldh;
+    void *Y; size_t ldy;
+    unsigned char *Q; size_t ldq;
+    unsigned char *S; size_t lds;
+    float *rstd;
+    const speech_drop *drop;
+} speech_norm;
+int speech_rows_rms_norm(int device, const speech_norm *args, void *stream);
+
+/* Its backward pass, from h and rstd as the forward pass left them, with g = dY weight:
+     dh = rstd g - h rstd^3 mean(g h) + dR;  dx = dropout(dh), the forward pass's mask;  dW = sum over rows of dY h rstd
+   dR      NULL, or the gradient that reaches h on the residual stream's own way.
+   dH      NULL, or gets dh rounded to dtype: the gradient of R, and of X where there was no dropout.  May be dY or dR.
+   dX      NULL, or gets dx (from dh in 32 bits).  May be dY or dR, unless dH is that one.
+   dW      NULL, or cols floats; then work points at work_bytes >= what speech_rows_rms_norm_work gives, on 16 bytes, that no other call in
+           flight uses (two captured graphs that may run at once need one each). */
+typedef struct speech_norm_grad {
+    int dtype, weight_f32;
+    size_t rows, cols;
+    const void *dY; size_t lddy;
+    const void *H; size_t ldh;
+    const float *rstd;
+    const void *weight;
+    const void *dR; size_t lddr;
+    void *dH; size_t lddh;
+    void *dX; size_t lddx;
+    float *dW;
+    const speech_drop *drop;
+    void *work; size_t work_bytes;
+} speech_norm_grad;
+int speech_rows_rms_norm_backward(int device, const speech_norm_grad *args, void *stream);
+int speech_rows_rms_norm_work(size_t rows, size_t cols, size_t *bytes);
+
+/* 8-bit form of a matrix: Q holds e4m3 values (4 exponent bits, 3 mantissa bits, largest 448, no infinities), S one byte e for each
+   block of 128 columns of a row, and element (i, j) stands for Q[i][j] 2^(S[i][j / 128] - 127).  A block's scale is the smallest
+   power of two (2^-127 at least) that brings its largest finite value to at most 448: a power of two costs a float format no
+   precision, is exact to divide by, and is what the matrix units apply by themselves.  Values are rounded to nearest, ties
+   to even; NaN and infinities become e4m3 NaN and leave their block's scale alone.
+   Rows of Q start on 16 bytes (Q and ldq are multiples of 16), rows of S on 4 (S and lds multiples of 4), and every row, the
+   last too, has memory behind it up to these multiples.  What stands there is neither read into a result nor written.
+   transpose != 0: the 8-bit form of X's transpose, cols rows of `rows` columns, blocks along X's rows: for the products that sum
+   over rows (gradients of weights). */
+int speech_rows_quantize(int device, int dtype, size_t rows, size_t cols, const void *X, size_t ldx, unsigned char *Q, size_t ldq,
+                         unsigned char *S, size_t lds, int transpose, void *stream);
+
+/* Y = A B^T + bias for two matrices in 8-bit form, A of rows x k, B of cols x k (a weight matrix with one row for each output, as it
+   is usually kept), summed in 32-bit floats and rounded once to dtype: SPEECH_BF16 or SPEECH_F16.  bias: NULL, or cols floats.
+   k == 0 gives the bias.  The matrix unit adds each eight products (columns 8 i ... 8 i + 7) at a resolution of 2^-13 of the largest of
+   them before they join the 32-bit sum: 1e-5 ... 4e-5 of a result as matrices of activations and weights have them, a tenth of a
+   16-bit type's own rounding, but no 32-bit result; there is none. */
+int speech_rows_product(int device, int dtype, size_t rows, size_t cols, size_t k, const unsigned char *A, size_t lda,
+                        const unsigned char *SA, size_t ldsa, const unsigned char *B, size_t ldb, const unsigned char *SB, size_t ldsb,
+                        const float *bias, void *Y, size_t ldy, void *stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SPEECH_AMD_LIB") or os.path.join(_HERE, "lib", "libspeech.so")   # the override is for A/B timing of builds
 
 KINDS = {"spectrogram": 0, "fbank": 1, "mfcc": 2, "plp": 3}
-F32, F64 = 0, 1
+F32, F64, BF16, F16 = 0, 1, 2, 3
 
 LEGACY_SYMBOLS = [
     "kaldi_fbank_s", "kaldi_fbank_d", "kaldi_fbank_default_s", "kaldi_fbank_default_d",
@@ -25,6 +25,8 @@ EXT_SYMBOLS = [
     "speech_batch_stats", "speech_batch_cmvn", "speech_batch_affine", "speech_batch_add_deltas", "speech_batch_splice",
     "speech_batch_splice_subsample", "speech_batch_subsample_rows", "speech_extract_pcm16", "speech_batch_set_ids", "speech_plan_run_host", "speech_host_release",
     "speech_batch_cmvn_noalloc", "speech_run_host_multi", "speech_shard_utterances", "speech_opts_frames", "speech_set_dropin_dither", "speech_batch_synth_audio", "speech_synth_audio_host",
+    "speech_batch_row_keys", "speech_rows_dropout", "speech_rows_rms_norm", "speech_rows_rms_norm_backward", "speech_rows_rms_norm_work",
+    "speech_rows_quantize", "speech_rows_product",
 ]
 
 
@@ -40,6 +42,27 @@ class SpeechOpts(C.Structure):
         ("compress", C.c_double), ("cep_scale", C.c_double), ("lpc_order", C.c_size_t),
         ("mn0", C.c_int), ("dither_seed", C.c_ulonglong), ("force_generic", C.c_int),
     ]
+
+
+class SpeechDrop(C.Structure):
+    """Mirror of `struct speech_drop`."""
+    _fields_ = [("p", C.c_double), ("seed", C.c_ulonglong), ("step", C.c_void_p), ("keys", C.c_void_p)]
+
+
+class SpeechNorm(C.Structure):
+    """Mirror of `struct speech_norm`."""
+    _fields_ = [("dtype", C.c_int), ("weight_f32", C.c_int), ("rows", C.c_size_t), ("cols", C.c_size_t), ("eps", C.c_double),
+                ("X", C.c_void_p), ("ldx", C.c_size_t), ("R", C.c_void_p), ("ldr", C.c_size_t), ("weight", C.c_void_p),
+                ("H", C.c_void_p), ("ldh", C.c_size_t), ("Y", C.c_void_p), ("ldy", C.c_size_t),
+                ("Q", C.c_void_p), ("ldq", C.c_size_t), ("S", C.c_void_p), ("lds", C.c_size_t), ("rstd", C.c_void_p), ("drop", C.POINTER(SpeechDrop))]
+
+
+class SpeechNormGrad(C.Structure):
+    """Mirror of `struct speech_norm_grad`."""
+    _fields_ = [("dtype", C.c_int), ("weight_f32", C.c_int), ("rows", C.c_size_t), ("cols", C.c_size_t),
+                ("dY", C.c_void_p), ("lddy", C.c_size_t), ("H", C.c_void_p), ("ldh", C.c_size_t), ("rstd", C.c_void_p), ("weight", C.c_void_p),
+                ("dR", C.c_void_p), ("lddr", C.c_size_t), ("dH", C.c_void_p), ("lddh", C.c_size_t), ("dX", C.c_void_p), ("lddx", C.c_size_t),
+                ("dW", C.c_void_p), ("drop", C.POINTER(SpeechDrop)), ("work", C.c_void_p), ("work_bytes", C.c_size_t)]
 
 
 _lib = None
@@ -108,6 +131,14 @@ def load():
     lib.speech_shard_utterances.argtypes = [z, C.POINTER(z), i, C.POINTER(i)]; lib.speech_shard_utterances.restype = i
     lib.speech_opts_frames.argtypes = [po, z, pz, pz]; lib.speech_opts_frames.restype = i
     lib.speech_extract_pcm16.argtypes = [C.POINTER(SpeechOpts), C.POINTER(C.c_short), z, vp]; lib.speech_extract_pcm16.restype = i
+    pdrop = C.POINTER(SpeechDrop)
+    lib.speech_batch_row_keys.argtypes = [vp, i, i, vp, vp]; lib.speech_batch_row_keys.restype = i
+    lib.speech_rows_dropout.argtypes = [i, i, z, z, vp, z, vp, z, pdrop, vp]; lib.speech_rows_dropout.restype = i
+    lib.speech_rows_rms_norm.argtypes = [i, C.POINTER(SpeechNorm), vp]; lib.speech_rows_rms_norm.restype = i
+    lib.speech_rows_rms_norm_backward.argtypes = [i, C.POINTER(SpeechNormGrad), vp]; lib.speech_rows_rms_norm_backward.restype = i
+    lib.speech_rows_rms_norm_work.argtypes = [z, z, pz]; lib.speech_rows_rms_norm_work.restype = i
+    lib.speech_rows_quantize.argtypes = [i, i, z, z, vp, z, vp, z, vp, z, i, vp]; lib.speech_rows_quantize.restype = i
+    lib.speech_rows_product.argtypes = [i, i, z, z, z, vp, z, vp, z, vp, z, vp, z, vp, vp, z, vp]; lib.speech_rows_product.restype = i
     _lib = lib
     return lib
 

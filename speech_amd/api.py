@@ -399,6 +399,12 @@ class Batch:
         self._check(self._lib.speech_batch_splice_subsample(self._h, _dev_ptr(Y, "Y", self.plan, self._y_end), _dev_ptr(Z, "Z", self.plan, need_z), int(left), int(right),
                                                             int(n), int(offset), C.c_void_p(stream) if stream else None))
 
+    def row_keys(self, keys, n=1, offset=0, stream=None):
+        """keys (int64, subsample_rows(n, offset)[1] elements) = what dropout keys the batch's rows by: utterance id << 32 | frame,
+        in the row order of splice_subsample (n = 1: of a dense batch)"""
+        need = self.subsample_rows(n, offset)[1]
+        self._check(self._lib.speech_batch_row_keys(self._h, int(n), int(offset), _dev_ptr(keys, "keys", self.plan, need, ("int64", "uint64")), C.c_void_p(stream) if stream else None))
+
     def close(self):
         if getattr(self, "_h", None):
             self._lib.speech_batch_destroy(self._h)
@@ -409,6 +415,194 @@ class Batch:
             self.close()
         except Exception:
             pass
+
+
+# ---- rows operators (include/speech_hip.h, speech_rows_*) on 2-D torch tensors with unit column stride ----
+#
+# All enqueue on `stream`, a raw hipStream_t value (e.g. torch.cuda.current_stream().cuda_stream; None: the device's default
+# stream), write into the tensors they are given and allocate nothing.  A tensor that torch may reuse before the stream gets to
+# the call has to be kept, or recorded on that stream, by the caller.
+
+_ROWS_TYPES = {"torch.float32": _lib.F32, "torch.bfloat16": _lib.BF16, "torch.float16": _lib.F16, "torch.float64": _lib.F64}
+_HELD = ("torch.uint8", "torch.float8_e4m3fn")
+_SCALES = ("torch.uint8", "torch.float8_e8m0fnu")
+
+
+def _rows_type(t, what, f64=False):
+    code = _ROWS_TYPES.get(str(t.dtype))
+    if code is None or (code == _lib.F64 and not f64):
+        raise ValueError("%s must have dtype float32, bfloat16%s, got %s" % (what, ", float16 or float64" if f64 else " or float16", t.dtype))
+    return code
+
+
+def _rows_arg(t, what, device, dtypes, rows, cols, pad=1):
+    """(pointer, row stride) of a rows x cols matrix after checking what the C ABI cannot: device, dtype, shape, strides, and that the
+    memory behind the last row reaches up to a multiple of `pad` columns"""
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError("%s must be on cuda:%d, got %s" % (what, device, t.device))
+    if str(t.dtype) not in dtypes:
+        raise ValueError("%s must have dtype %s, got %s" % (what, " or ".join(d[6:] for d in dtypes), t.dtype))
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise ValueError("%s must have shape (%d, %d), got %s" % (what, rows, cols, tuple(t.shape)))
+    ld, unit = t.stride()
+    if cols > 1 and unit != 1:
+        raise ValueError("%s must have unit column stride, got %d" % (what, unit))
+    full = -(-cols // pad) * pad
+    if rows <= 1 or cols == 0:
+        ld = full
+    elif ld < cols or (pad > 1 and ld % pad):
+        raise ValueError("%s has a row stride of %d for %d columns%s" % (what, ld, cols, "" if pad == 1 else ": a multiple of %d is needed" % pad))
+    if pad > 1 and rows and cols:
+        if t.storage_offset() + (rows - 1) * ld + full > t.untyped_storage().nbytes() or t.data_ptr() % pad:
+            raise ValueError("%s needs rows that start on %d bytes and have memory up to the next %d (see held)" % (what, pad, pad))
+    return t.data_ptr(), ld
+
+
+def _vector_arg(t, what, device, dtypes, n):
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError("%s must be on cuda:%d, got %s" % (what, device, t.device))
+    if str(t.dtype) not in dtypes:
+        raise ValueError("%s must have dtype %s, got %s" % (what, " or ".join(d[6:] for d in dtypes), t.dtype))
+    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError("%s must be a contiguous vector of %d elements, got %s" % (what, n, tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _drop_arg(p, seed, step, keys, device, rows):
+    """speech_drop, or None where nothing is dropped"""
+    p = float(p)
+    if p == 0.0:
+        return None
+    d = _lib.SpeechDrop(p, int(seed) & 0xFFFFFFFFFFFFFFFF, None, None)
+    if step is not None:
+        d.step = _vector_arg(step.reshape(-1), "step", device, ("torch.int64", "torch.uint64"), 1)
+    if keys is not None:
+        d.keys = _vector_arg(keys, "keys", device, ("torch.int64", "torch.uint64"), rows)
+    return d
+
+
+def _rows_check(rc):
+    if rc != 0:
+        raise SpeechError(_lib.last_error())
+
+
+def held(rows, cols, device="cuda"):
+    """(Q, S): room for a rows x cols matrix in 8-bit form, with the padding that the operators need: e4m3 values whose rows start on
+    16 bytes, and a scale byte for each block of 128 columns, rows of them on 4 bytes"""
+    import torch
+    nb = -(-cols // 128)
+    q = torch.zeros(rows, -(-cols // 16) * 16, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
+    return q, torch.zeros(rows, -(-nb // 4) * 4, dtype=torch.uint8, device=device)[:, :nb]
+
+
+def dropout(X, Y, p, seed, step=None, keys=None, stream=None):
+    """Y = X / (1 - p) where 32 random bits keyed by (seed + step, keys[row], column) say so, else 0; Y may be X.  The same call
+    on a gradient is the backward pass.  step: an int64 tensor of one element on the device, added to the seed when the kernel runs"""
+    code = _rows_type(X, "X", f64=True)
+    rows, cols = X.shape
+    dev = X.get_device()
+    xp, ldx = _rows_arg(X, "X", dev, (str(X.dtype),), rows, cols)
+    yp, ldy = _rows_arg(Y, "Y", dev, (str(X.dtype),), rows, cols)
+    d = _drop_arg(p, seed, step, keys, dev, rows) or _lib.SpeechDrop(0.0, 0, None, None)
+    _rows_check(_lib.load().speech_rows_dropout(dev, code, rows, cols, xp, ldx, yp, ldy, C.byref(d), stream or None))
+
+
+def rms_norm(X, weight=None, eps=1e-6, residual=None, H=None, Y=None, Q=None, S=None, rstd=None, p=0.0, seed=0, step=None, keys=None, stream=None):
+    """h = residual + dropout(X) -> H; h / sqrt(mean(h^2) + eps) * weight -> Y, or in 8-bit form -> (Q, S); 1 / sqrt(...) -> rstd.
+    weight: X's dtype or float32.  H may be X or residual (in place)"""
+    code = _rows_type(X, "X")
+    rows, cols = X.shape
+    dev = X.get_device()
+    same = (str(X.dtype),)
+    a = _lib.SpeechNorm(dtype=code, rows=rows, cols=cols, eps=float(eps))
+    a.X, a.ldx = _rows_arg(X, "X", dev, same, rows, cols)
+    if residual is not None:
+        a.R, a.ldr = _rows_arg(residual, "residual", dev, same, rows, cols)
+    if weight is not None:
+        a.weight = _vector_arg(weight, "weight", dev, same + ("torch.float32",), cols)
+        a.weight_f32 = int(str(weight.dtype) == "torch.float32")
+    if H is not None:
+        a.H, a.ldh = _rows_arg(H, "H", dev, same, rows, cols)
+    if Y is not None:
+        a.Y, a.ldy = _rows_arg(Y, "Y", dev, same, rows, cols)
+    if Q is not None:
+        if S is None:
+            raise ValueError("Q needs S")
+        a.Q, a.ldq = _rows_arg(Q, "Q", dev, _HELD, rows, cols, 16)
+        a.S, a.lds = _rows_arg(S, "S", dev, _SCALES, rows, -(-cols // 128), 4)
+    if rstd is not None:
+        a.rstd = _vector_arg(rstd, "rstd", dev, ("torch.float32",), rows)
+    d = _drop_arg(p, seed, step, keys, dev, rows)
+    if d is not None:
+        a.drop = C.pointer(d)
+    _rows_check(_lib.load().speech_rows_rms_norm(dev, C.byref(a), stream or None))
+
+
+def rms_norm_work(rows, cols):
+    """bytes of `work` that rms_norm_backward needs for dW"""
+    n = C.c_size_t()
+    _rows_check(_lib.load().speech_rows_rms_norm_work(int(rows), int(cols), C.byref(n)))
+    return n.value
+
+
+def rms_norm_backward(dY, H, weight, rstd, dH=None, dR=None, dX=None, dW=None, work=None, p=0.0, seed=0, step=None, keys=None, stream=None):
+    """gradients of rms_norm from dY, the H and rstd it left, and dR, what reaches H on the residual stream's own way: dH (of the
+    residual stream; of X where nothing was dropped), dX (of the dropped X), dW (float32).  work: a uint8 tensor of
+    rms_norm_work(rows, cols) bytes at least, not used by another call in flight"""
+    code = _rows_type(H, "H")
+    rows, cols = H.shape
+    dev = H.get_device()
+    same = (str(H.dtype),)
+    a = _lib.SpeechNormGrad(dtype=code, rows=rows, cols=cols)
+    a.dY, a.lddy = _rows_arg(dY, "dY", dev, same, rows, cols)
+    a.H, a.ldh = _rows_arg(H, "H", dev, same, rows, cols)
+    a.rstd = _vector_arg(rstd, "rstd", dev, ("torch.float32",), rows)
+    if weight is not None:
+        a.weight = _vector_arg(weight, "weight", dev, same + ("torch.float32",), cols)
+        a.weight_f32 = int(str(weight.dtype) == "torch.float32")
+    if dR is not None:
+        a.dR, a.lddr = _rows_arg(dR, "dR", dev, same, rows, cols)
+    if dH is not None:
+        a.dH, a.lddh = _rows_arg(dH, "dH", dev, same, rows, cols)
+    if dX is not None:
+        a.dX, a.lddx = _rows_arg(dX, "dX", dev, same, rows, cols)
+    if dW is not None:
+        a.dW = _vector_arg(dW, "dW", dev, ("torch.float32",), cols)
+        if work is not None:
+            a.work, a.work_bytes = _vector_arg(work, "work", dev, ("torch.uint8",), work.numel()), work.numel()
+    d = _drop_arg(p, seed, step, keys, dev, rows)
+    if d is not None:
+        a.drop = C.pointer(d)
+    _rows_check(_lib.load().speech_rows_rms_norm_backward(dev, C.byref(a), stream or None))
+
+
+def quantize(X, Q, S, transpose=False, stream=None):
+    """(Q, S) = X in 8-bit form (see held): e4m3 values and a power-of-two scale for each 128 columns; transpose: X's transpose"""
+    code = _rows_type(X, "X")
+    rows, cols = X.shape
+    dev = X.get_device()
+    xp, ldx = _rows_arg(X, "X", dev, (str(X.dtype),), rows, cols)
+    r, c = (cols, rows) if transpose else (rows, cols)
+    qp, ldq = _rows_arg(Q, "Q", dev, _HELD, r, c, 16)
+    sp, lds = _rows_arg(S, "S", dev, _SCALES, r, -(-c // 128), 4)
+    _rows_check(_lib.load().speech_rows_quantize(dev, code, rows, cols, xp, ldx, qp, ldq, sp, lds, int(bool(transpose)), stream or None))
+
+
+def product(A, SA, B, SB, Y, bias=None, stream=None):
+    """Y = A B^T + bias for A (rows x k) and B (columns x k, a weight matrix with a row for each output) in 8-bit form; Y bfloat16 or
+    float16, bias float32"""
+    code = _rows_type(Y, "Y")                                  # float32 is refused by the C side
+    rows, cols = Y.shape
+    k = A.shape[1]
+    dev = Y.get_device()
+    nb = -(-k // 128)
+    ap, lda = _rows_arg(A, "A", dev, _HELD, rows, k, 16)
+    sa, ldsa = _rows_arg(SA, "SA", dev, _SCALES, rows, nb, 4)
+    bp, ldb = _rows_arg(B, "B", dev, _HELD, cols, k, 16)
+    sb, ldsb = _rows_arg(SB, "SB", dev, _SCALES, cols, nb, 4)
+    yp, ldy = _rows_arg(Y, "Y", dev, (str(Y.dtype),), rows, cols)
+    bias_p = _vector_arg(bias, "bias", dev, ("torch.float32",), cols) if bias is not None else None
+    _rows_check(_lib.load().speech_rows_product(dev, code, rows, cols, k, ap, lda, sa, ldsa, bp, ldb, sb, ldsb, bias_p, yp, ldy, stream or None))
 
 
 def merge_stats(s, q, n, group=None):

@@ -1,0 +1,163 @@
+// rows_internal.hpp -- what the rows operators' host layer (rows_api.hip) and kernels (rows_kernels.hip, rows_product.hip) share.
+#pragma once
+#include "speech_internal.hpp"
+
+namespace speech {
+
+constexpr int ROWS_BLOCK = 128;                 // columns that share a scale: one k-step of the 16x16x128 matrix instruction
+constexpr int ROWS_GRAD_MAX_WG = 1024;          // partial sums of the weight's gradient
+
+struct DropParams {
+    int on;
+    uint32_t thresh;                            // floor(p 2^32)
+    double scale;                               // 1 / (1 - p)
+    unsigned long long seed;
+    const unsigned long long *step, *keys;
+};
+
+struct NormParams {
+    size_t rows;
+    int cols, weight_f32;
+    float eps;
+    const void *X, *R, *weight;
+    void *H, *Y;
+    size_t ldx, ldr, ldh, ldy;
+    uint8_t *Q, *S;
+    size_t ldq, lds;
+    float *rstd;
+    DropParams drop;
+};
+
+struct NormGradParams {
+    size_t rows;
+    int cols, weight_f32;
+    const void *dY, *H, *dR, *weight;
+    const float *rstd;
+    void *dH, *dX;
+    size_t lddy, ldh, lddr, lddh, lddx;
+    float *dW, *work;
+    DropParams drop;
+};
+
+struct ProductParams {
+    size_t M, N, K;
+    const uint8_t *A, *SA, *B, *SB;
+    size_t lda, ldsa, ldb, ldsb;
+    const float *bias;
+    void *Y;
+    size_t ldy;
+};
+
+hipError_t launch_row_keys(const UttDesc *utts, uint32_t nutt, const TileDesc *tiles, uint32_t ntiles, int n, int offset,
+                           unsigned long long *base, unsigned long long *keys, hipStream_t s);
+hipError_t launch_rows_dropout(int dtype, size_t rows, int cols, const void *X, size_t ldx, void *Y, size_t ldy, const DropParams &d, hipStream_t s);
+hipError_t launch_rows_norm(int dtype, const NormParams &p, hipStream_t s);
+hipError_t launch_rows_norm_grad(int dtype, const NormGradParams &p, hipStream_t s);
+hipError_t launch_rows_quantize(int dtype, size_t rows, size_t cols, const void *X, size_t ldx, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds,
+                                int transpose, hipStream_t s);
+hipError_t launch_rows_product(int dtype, const ProductParams &p, hipStream_t s);
+
+#if defined(__HIPCC__)
+template <typename T> constexpr int vec_of() { return 16 / (int)sizeof(T); }
+// vectors of 16 bytes at any address a T may have: the device reads and writes them whole wherever they start
+template <typename T, int N> struct VecOf { typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T)))); };
+
+// the n <= N elements at p, as F; the rest 0
+template <typename F, typename T, int N>
+__device__ __forceinline__ void load_vals(const T *p, int n, F (&v)[N])
+{
+    if (n >= N)
+    {
+        const typename VecOf<T, N>::type x = *reinterpret_cast<const typename VecOf<T, N>::type *>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) { v[i] = (F)x[i]; }
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { v[i] = i < n ? (F)p[i] : (F)0; }
+    }
+}
+
+template <typename F, typename T, int N>
+__device__ __forceinline__ void store_vals(T *p, int n, const F (&v)[N])
+{
+    if (n >= N)
+    {
+        typename VecOf<T, N>::type x;
+#pragma unroll
+        for (int i = 0; i < N; ++i) { x[i] = (T)v[i]; }
+        *reinterpret_cast<typename VecOf<T, N>::type *>(p) = x;
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { if (i < n) { p[i] = (T)v[i]; } }
+    }
+}
+
+// ---- 8-bit form ----
+// Largest finite magnitude as float bits (unsigned order is magnitude order); NaN and infinities count as 0.
+__device__ __forceinline__ unsigned finite_bits(float v)
+{
+    const unsigned u = __float_as_uint(v) & 0x7FFFFFFFu;
+    return u < 0x7F800000u ? u : 0u;
+}
+// Biased exponent of the smallest power of two that brings amax = m 2^E, 1 <= m < 2, to at most 448 = 1.75 2^8:
+// 2^(E - 8), or twice that where m > 1.75; from the bits of amax, 2^-127 at least.
+__device__ __forceinline__ unsigned block_exponent(unsigned amax)
+{
+    const int e = (int)(amax >> 23) - 8 + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e > 0 ? (unsigned)e : 0u;
+}
+// 2^(127 - s), 2^127 ... 2^-120: a normal number for every s that block_exponent returns (0 ... 247)
+__device__ __forceinline__ float block_factor(unsigned s) { return __uint_as_float((254u - s) << 23); }
+// four values of a block, already times its factor, to e4m3, nearest even; what is no finite number becomes NaN
+__device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d)
+{
+    const float big = __uint_as_float(0x7FC00000u);
+    a = fabsf(a) <= 448.0f ? a : big; b = fabsf(b) <= 448.0f ? b : big;
+    c = fabsf(c) <= 448.0f ? c : big; d = fabsf(d) <= 448.0f ? d : big;
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// ---- reductions over the 16 lanes of a DPP row, then over the wave ----
+template <int CTRL> __device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140;
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v += __uint_as_float(dpp<DPP_XOR1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<DPP_XOR2>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<DPP_HALF_MIRROR>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<DPP_MIRROR>(__float_as_uint(v)));
+    if (LANES >= 32) { v += __shfl_xor(v, 16); }
+    if (LANES >= 64) { v += __shfl_xor(v, 32); }
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_max(unsigned v)
+{
+    v = max(v, dpp<DPP_XOR1>(v));
+    v = max(v, dpp<DPP_XOR2>(v));
+    v = max(v, dpp<DPP_HALF_MIRROR>(v));
+    if (LANES >= 16) { v = max(v, dpp<DPP_MIRROR>(v)); }
+    if (LANES >= 32) { v = max(v, (unsigned)__shfl_xor((int)v, 16)); }
+    return v;
+}
+
+// ---- dropout's generator: the dither's hash (speech_internal.hpp) under a key of its own ----
+constexpr unsigned long long DROP_DOMAIN = 0xD1B54A32D192ED03ull;
+__device__ __forceinline__ unsigned long long drop_layer_key(const DropParams &d)
+{
+    return mix64((d.seed + (d.step ? *d.step : 0ull)) ^ DROP_DOMAIN);
+}
+__device__ __forceinline__ unsigned long long drop_row_key(unsigned long long ku, const DropParams &d, size_t row)
+{
+    return mix64(ku ^ (d.keys ? d.keys[row] : (unsigned long long)row));
+}
+__device__ __forceinline__ bool drop_keeps(unsigned long long fk, unsigned col, unsigned thresh) { return dither_bits(fk, col) >= thresh; }
+#endif
+
+}  // namespace speech

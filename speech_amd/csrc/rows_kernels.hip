@@ -1,0 +1,658 @@
+// rows_kernels.hip -- dropout, RMS norm (forward, backward, 8-bit output) and the 8-bit quantizer on frame-major matrices, gfx950.
+//
+// All are passes over rows that HBM bounds: every element is read once and written once, in vectors of 16 bytes a lane, and what
+// a row needs in between (sum of squares, block maxima, the mask) stays in registers.
+#include "rows_internal.hpp"
+
+namespace speech {
+namespace {
+
+constexpr int NT = 256;
+
+template <typename F> struct Compute { typedef float type; };
+template <> struct Compute<double> { typedef double type; };
+
+// ---- keys of a batch's rows ----
+// base[u] = rows of the utterances before u, ceil((W - offset) / n) each: one workgroup scans the utterances 1024 at a time.
+__global__ __launch_bounds__(1024) void row_base_kernel(const UttDesc *utts, uint32_t nutt, int n, int offset, unsigned long long *base)
+{
+    __shared__ unsigned long long sh[1024];
+    unsigned long long before = 0;
+    const int t = threadIdx.x;
+    for (uint32_t u0 = 0; u0 < nutt; u0 += 1024)
+    {
+        const uint32_t u = u0 + t;
+        const unsigned long long W = u < nutt ? utts[u].W : 0ull;
+        const unsigned long long r = W > (unsigned long long)offset ? (W - offset + n - 1) / n : 0ull;
+        unsigned long long sum = r;
+        sh[t] = sum;
+        __syncthreads();
+        for (int d = 1; d < 1024; d *= 2)
+        {
+            const unsigned long long o = t >= d ? sh[t - d] : 0ull;
+            __syncthreads();
+            sum += o; sh[t] = sum;
+            __syncthreads();
+        }
+        if (u < nutt) { base[u] = before + sum - r; }
+        before += sh[1023];
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(64) void row_keys_kernel(const TileDesc *tiles, int n, int offset, const unsigned long long *base, unsigned long long *keys)
+{
+    const TileDesc tile = tiles[blockIdx.x];
+    for (uint32_t i = threadIdx.x; i < tile.nframes; i += 64)
+    {
+        const unsigned long long w = (unsigned long long)tile.frame0 + i;
+        if (w >= (unsigned long long)offset && (w - offset) % n == 0) { keys[base[tile.utt] + (w - offset) / n] = (unsigned long long)tile.uid << 32 | w; }
+    }
+}
+
+// ---- dropout ----
+// A thread takes vectors of a row's elements (the last of a row may be short), a grid's width apart; row and place move by fixed
+// steps, so that nothing is divided inside the loop.
+template <typename T>
+__global__ __launch_bounds__(NT) void dropout_kernel(const T *X, T *Y, size_t ldx, size_t ldy, size_t rows, int cols, int nv, size_t step_row, int step_v,
+                                                     const DropParams d)
+{
+    typedef typename Compute<T>::type F;
+    constexpr int N = vec_of<T>();
+    const unsigned long long ku = drop_layer_key(d);
+    const size_t first = (size_t)blockIdx.x * NT + threadIdx.x;
+    size_t row = first / (unsigned)nv;
+    int v = (int)(first - row * (unsigned)nv);
+    const F scale = (F)d.scale;
+    while (row < rows)
+    {
+        const int c = v * N;
+        F x[N];
+        load_vals<F>(X + row * ldx + c, cols - c, x);
+        if (d.on)
+        {
+            const unsigned long long fk = drop_row_key(ku, d, row);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { x[i] = drop_keeps(fk, (unsigned)(c + i), d.thresh) ? x[i] * scale : (F)0; }
+        }
+        store_vals(Y + row * ldy + c, cols - c, x);
+        row += step_row; v += step_v;
+        if (v >= nv) { v -= nv; ++row; }
+    }
+}
+
+// ---- RMS norm ----
+// Sum over the TPR threads of a row.  TPR <= 64: lanes of one wave.  Above: a partial of each wave in LDS, added in wave order by
+// everybody; sh is used twice in turn (flip), so that one barrier a row is enough.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *sh, int &flip)
+{
+    if (TPR <= 64) { return lanes_sum<TPR>(v); }
+    constexpr int W = TPR > 64 ? TPR / 64 : 1;
+    v = lanes_sum<64>(v);
+    float *s = sh + flip * W;
+    flip ^= 1;
+    if ((threadIdx.x & 63) == 0) { s[threadIdx.x >> 6] = v; }
+    __syncthreads();
+    float t = s[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) { t += s[w]; }
+    return t;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void load_weight(const void *w, int f32, int c, int n, float (&v)[N])
+{
+    if (!w)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { v[i] = 1.0f; }
+    }
+    else if (f32)
+    {
+        if (n >= N)
+        {
+#pragma unroll
+            for (int i = 0; i < N; i += 4)
+            {
+                const VecOf<float, 4>::type x = *reinterpret_cast<const VecOf<float, 4>::type *>(reinterpret_cast<const float *>(w) + c + i);
+                v[i] = x[0]; v[i + 1] = x[1]; v[i + 2] = x[2]; v[i + 3] = x[3];
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i) { v[i] = i < n ? reinterpret_cast<const float *>(w)[c + i] : 0.0f; }
+        }
+    }
+    else { load_vals<float>(reinterpret_cast<const T *>(w) + c, n, v); }
+}
+
+// h = R + dropout(X) of N elements, rounded to T (what follows uses the rounded values, as the backward pass will)
+template <typename T, int N>
+__device__ __forceinline__ void norm_input(const NormParams &p, size_t row, int c, unsigned long long fk, float (&h)[N])
+{
+    const int n = p.cols - c;
+    load_vals<float>(reinterpret_cast<const T *>(p.X) + row * p.ldx + c, n, h);
+    if (p.drop.on)
+    {
+        const float scale = (float)p.drop.scale;
+#pragma unroll
+        for (int i = 0; i < N; ++i) { h[i] = drop_keeps(fk, (unsigned)(c + i), p.drop.thresh) ? h[i] * scale : 0.0f; }
+    }
+    if (p.R)
+    {
+        float r[N];
+        load_vals<float>(reinterpret_cast<const T *>(p.R) + row * p.ldr + c, n, r);
+#pragma unroll
+        for (int i = 0; i < N; ++i) { h[i] += r[i]; }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) { h[i] = (float)(T)h[i]; }
+}
+
+__device__ __forceinline__ float rstd_of(float ss, const NormParams &p) { return 1.0f / sqrtf(ss / (float)p.cols + p.eps); }
+
+template <int N>
+__device__ __forceinline__ void store_e4m3(uint8_t *q, int n, const float (&y)[N], float f)
+{
+    unsigned w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) { w[i] = pack_e4m3(y[4 * i] * f, y[4 * i + 1] * f, y[4 * i + 2] * f, y[4 * i + 3] * f); }
+    if (n >= N)
+    {
+        if (N == 8) { *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[N / 4 - 1]); }
+        else { *reinterpret_cast<unsigned *>(q) = w[0]; }
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { if (i < n) { q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4))); } }
+    }
+}
+
+// A row stays in the registers of its TPR threads, CH vectors each, from its one reading to its one writing.
+template <typename T, int TPR, int CH>
+__global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormParams p)
+{
+    constexpr int N = vec_of<T>(), NTH = TPR > NT ? TPR : NT, RPW = NTH / TPR, LB = ROWS_BLOCK / N;
+    __shared__ float sh[2 * (NTH / 64)];
+    const int t = threadIdx.x % TPR;
+    int flip = 0;
+    const unsigned long long ku = drop_layer_key(p.drop);
+    const int nb = (p.cols + ROWS_BLOCK - 1) / ROWS_BLOCK;
+    for (size_t row = (size_t)blockIdx.x * RPW + threadIdx.x / TPR; row < p.rows; row += (size_t)gridDim.x * RPW)
+    {
+        const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
+        float h[CH][N];
+        float ss = 0.0f;
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+            const int c = (k * TPR + t) * N;
+            norm_input<T>(p, row, c, fk, h[k]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { ss += c + i < p.cols ? h[k][i] * h[k][i] : 0.0f; }
+        }
+        if (p.H)
+        {
+#pragma unroll
+            for (int k = 0; k < CH; ++k)
+            {
+                const int c = (k * TPR + t) * N;
+                store_vals(reinterpret_cast<T *>(p.H) + row * p.ldh + c, p.cols - c, h[k]);
+            }
+        }
+        const float rstd = rstd_of(row_sum<TPR>(ss, sh, flip), p);
+        if (p.rstd && t == 0) { p.rstd[row] = rstd; }
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+            const int c = (k * TPR + t) * N;
+            float w[N];
+            load_weight<T>(p.weight, p.weight_f32, c, p.cols - c, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { h[k][i] = h[k][i] * rstd * w[i]; }
+            if (p.Y) { store_vals(reinterpret_cast<T *>(p.Y) + row * p.ldy + c, p.cols - c, h[k]); }
+        }
+        if (p.Q)
+        {
+            unsigned amax[CH];
+#pragma unroll
+            for (int k = 0; k < CH; ++k)
+            {
+                amax[k] = 0u;
+#pragma unroll
+                for (int i = 0; i < N; ++i) { amax[k] = max(amax[k], (k * TPR + t) * N + i < p.cols ? finite_bits(h[k][i]) : 0u); }
+            }
+            if (TPR < LB)                                                    // the whole row is one block
+            {
+#pragma unroll
+                for (int k = 1; k < CH; ++k) { amax[0] = max(amax[0], amax[k]); }
+                amax[0] = lanes_max<16>(amax[0]);
+#pragma unroll
+                for (int k = 1; k < CH; ++k) { amax[k] = amax[0]; }
+            }
+            else
+            {
+#pragma unroll
+                for (int k = 0; k < CH; ++k) { amax[k] = lanes_max<LB>(amax[k]); }
+            }
+#pragma unroll
+            for (int k = 0; k < CH; ++k)
+            {
+                const int c = (k * TPR + t) * N;
+                const unsigned e = block_exponent(amax[k]);
+                store_e4m3(p.Q + row * p.ldq + c, p.cols - c, h[k], block_factor(e));
+                const int b = c / ROWS_BLOCK;
+                if (c % ROWS_BLOCK == 0 && b < nb) { p.S[row * p.lds + b] = (uint8_t)e; }
+            }
+        }
+    }
+}
+
+// Rows of any width: a workgroup walks its row twice; the second time H if it was written, which may have replaced X or R.
+template <typename T>
+__global__ __launch_bounds__(NT) void norm_wide_kernel(const NormParams p)
+{
+    constexpr int N = vec_of<T>(), LB = ROWS_BLOCK / N;
+    __shared__ float sh[2 * (NT / 64)];
+    int flip = 0;
+    const unsigned long long ku = drop_layer_key(p.drop);
+    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x)
+    {
+        const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
+        float ss = 0.0f;
+        for (int c = threadIdx.x * N; c < p.cols; c += NT * N)
+        {
+            float h[N];
+            norm_input<T>(p, row, c, fk, h);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { ss += c + i < p.cols ? h[i] * h[i] : 0.0f; }
+            if (p.H) { store_vals(reinterpret_cast<T *>(p.H) + row * p.ldh + c, p.cols - c, h); }
+        }
+        const float rstd = rstd_of(row_sum<NT>(ss, sh, flip), p);
+        if (p.rstd && threadIdx.x == 0) { p.rstd[row] = rstd; }
+        const int padded = (p.cols + ROWS_BLOCK - 1) / ROWS_BLOCK * ROWS_BLOCK;   // whole blocks: all lanes of a block take part in its maximum
+        for (int c = threadIdx.x * N; c < padded; c += NT * N)
+        {
+            float h[N], w[N];
+            if (p.H) { load_vals<float>(reinterpret_cast<const T *>(p.H) + row * p.ldh + c, p.cols - c, h); }
+            else { norm_input<T>(p, row, c, fk, h); }
+            load_weight<T>(p.weight, p.weight_f32, c, p.cols - c, w);
+            unsigned amax = 0u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) { h[i] = h[i] * rstd * w[i]; amax = max(amax, c + i < p.cols ? finite_bits(h[i]) : 0u); }
+            if (p.Y) { store_vals(reinterpret_cast<T *>(p.Y) + row * p.ldy + c, p.cols - c, h); }
+            if (p.Q)
+            {
+                const unsigned e = block_exponent(lanes_max<LB>(amax));
+                store_e4m3(p.Q + row * p.ldq + c, p.cols - c, h, block_factor(e));
+                if (c % ROWS_BLOCK == 0) { p.S[row * p.lds + c / ROWS_BLOCK] = (uint8_t)e; }
+            }
+        }
+    }
+}
+
+// ---- backward ----
+// g = dY w of N elements; returns dY h summed with the weight: what the row's mean takes
+template <typename T, int N>
+__device__ __forceinline__ float grad_input(const NormGradParams &p, size_t row, int c, float (&dy)[N], float (&h)[N], float (&g)[N])
+{
+    const int n = p.cols - c;
+    load_vals<float>(reinterpret_cast<const T *>(p.dY) + row * p.lddy + c, n, dy);
+    load_vals<float>(reinterpret_cast<const T *>(p.H) + row * p.ldh + c, n, h);
+    load_weight<T>(p.weight, p.weight_f32, c, n, g);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { g[i] *= dy[i]; s += i < n ? g[i] * h[i] : 0.0f; }
+    return s;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void grad_output(const NormGradParams &p, size_t row, int c, unsigned long long fk, float rstd, float coef, const float (&h)[N], float (&g)[N])
+{
+    const int n = p.cols - c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) { g[i] = g[i] * rstd - h[i] * coef; }
+    if (p.dR)
+    {
+        float r[N];
+        load_vals<float>(reinterpret_cast<const T *>(p.dR) + row * p.lddr + c, n, r);
+#pragma unroll
+        for (int i = 0; i < N; ++i) { g[i] += r[i]; }
+    }
+    if (p.dH) { store_vals(reinterpret_cast<T *>(p.dH) + row * p.lddh + c, n, g); }
+    if (p.dX)
+    {
+        if (p.drop.on)
+        {
+            const float scale = (float)p.drop.scale;
+#pragma unroll
+            for (int i = 0; i < N; ++i) { g[i] = drop_keeps(fk, (unsigned)(c + i), p.drop.thresh) ? g[i] * scale : 0.0f; }
+        }
+        store_vals(reinterpret_cast<T *>(p.dX) + row * p.lddx + c, n, g);
+    }
+}
+
+// As the forward kernel; besides, every thread keeps the sums over its rows of dY h rstd for its columns.  At the end a workgroup
+// adds its row groups' sums in group order and leaves one row of partial sums in `work`: no atomics, the same sums every time.
+template <typename T, int TPR, int CH>
+__global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_grad_kernel(const NormGradParams p)
+{
+    constexpr int N = vec_of<T>(), NTH = TPR > NT ? TPR : NT, RPW = NTH / TPR;
+    __shared__ float sh[2 * (NTH / 64)];
+    __shared__ float part[RPW > 1 ? NTH * N : 1];
+    const int t = threadIdx.x % TPR;
+    int flip = 0;
+    const unsigned long long ku = drop_layer_key(p.drop);
+    float acc[CH][N];
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { acc[k][i] = 0.0f; }
+    }
+    for (size_t row = (size_t)blockIdx.x * RPW + threadIdx.x / TPR; row < p.rows; row += (size_t)gridDim.x * RPW)
+    {
+        const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
+        const float rstd = p.rstd[row];
+        float h[CH][N], g[CH][N];
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+            float dy[N];
+            s += grad_input<T>(p, row, (k * TPR + t) * N, dy, h[k], g[k]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { acc[k][i] += dy[i] * (h[k][i] * rstd); }
+        }
+        const float mean = row_sum<TPR>(s, sh, flip) / (float)p.cols;
+        const float coef = mean * rstd * rstd * rstd;
+#pragma unroll
+        for (int k = 0; k < CH; ++k) { grad_output<T>(p, row, (k * TPR + t) * N, fk, rstd, coef, h[k], g[k]); }
+    }
+    if (!p.dW) { return; }
+    float *out = p.work + (size_t)blockIdx.x * p.cols;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+    {
+        const int c = (k * TPR + t) * N;
+        if (RPW > 1)
+        {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i) { part[i * NTH + threadIdx.x] = acc[k][i]; }
+            __syncthreads();
+            if (threadIdx.x < TPR)
+            {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                {
+                    float s = part[i * NTH + t];
+                    for (int r = 1; r < RPW; ++r) { s += part[i * NTH + r * TPR + t]; }
+                    acc[k][i] = s;
+                }
+            }
+        }
+        if (threadIdx.x < TPR) { store_vals(out + c, p.cols - c, acc[k]); }
+    }
+}
+
+// Rows of any width: dH and dX by a workgroup a row, walked twice; the weight's partial sums by norm_grad_weight_kernel before it,
+// since dH may replace dY.
+template <typename T>
+__global__ __launch_bounds__(NT) void norm_grad_wide_kernel(const NormGradParams p)
+{
+    constexpr int N = vec_of<T>();
+    __shared__ float sh[2 * (NT / 64)];
+    int flip = 0;
+    const unsigned long long ku = drop_layer_key(p.drop);
+    for (size_t row = blockIdx.x; row < p.rows; row += gridDim.x)
+    {
+        const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
+        const float rstd = p.rstd[row];
+        float s = 0.0f;
+        for (int c = threadIdx.x * N; c < p.cols; c += NT * N)
+        {
+            float dy[N], h[N], g[N];
+            s += grad_input<T>(p, row, c, dy, h, g);
+        }
+        const float coef = row_sum<NT>(s, sh, flip) / (float)p.cols * rstd * rstd * rstd;
+        for (int c = threadIdx.x * N; c < p.cols; c += NT * N)
+        {
+            float dy[N], h[N], g[N];
+            (void)grad_input<T>(p, row, c, dy, h, g);
+            grad_output<T>(p, row, c, fk, rstd, coef, h, g);
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void norm_grad_weight_kernel(const NormGradParams p, int groups)
+{
+    const int c = blockIdx.x * NT + threadIdx.x;
+    if (c >= p.cols) { return; }
+    float s = 0.0f;
+    for (size_t row = blockIdx.y; row < p.rows; row += groups)
+    {
+        s += (float)reinterpret_cast<const T *>(p.dY)[row * p.lddy + c] * ((float)reinterpret_cast<const T *>(p.H)[row * p.ldh + c] * p.rstd[row]);
+    }
+    p.work[(size_t)blockIdx.y * p.cols + c] = s;
+}
+
+// dW[c] = sum of the groups' partial sums: 32 columns a workgroup, 8 threads for each take every 8th group, their sums are added in
+// order
+__global__ __launch_bounds__(NT) void norm_grad_reduce_kernel(const float *work, float *dW, int cols, int groups)
+{
+    __shared__ float sh[NT];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+    float s = 0.0f;
+    if (c < cols) { for (int g = k; g < groups; g += 8) { s += work[(size_t)g * cols + c]; } }
+    sh[threadIdx.x] = s;
+    __syncthreads();
+    if (k == 0 && c < cols)
+    {
+        for (int j = 1; j < 8; ++j) { s += sh[j * 32 + threadIdx.x]; }
+        dW[c] = s;
+    }
+}
+
+// ---- the quantizer ----
+// 16 lanes take a block of a row, 8 elements each.
+template <typename T>
+__global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, size_t rows, size_t cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, size_t nb)
+{
+    const size_t units = rows * nb;
+    const int l = threadIdx.x & 15;
+    for (size_t u = (size_t)blockIdx.x * (NT / 16) + threadIdx.x / 16; u < units; u += (size_t)gridDim.x * (NT / 16))
+    {
+        const size_t row = u / nb, b = u - row * nb, c = b * ROWS_BLOCK + l * 8;
+        const int n = c < cols ? (int)min(cols - c, (size_t)8) : 0;
+        float x[8];
+        load_vals<float>(X + row * ldx + c, n, x);
+        unsigned amax = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { amax = max(amax, finite_bits(x[i])); }
+        const unsigned e = block_exponent(lanes_max<16>(amax));
+        store_e4m3(Q + row * ldq + c, n, x, block_factor(e));
+        if (l == 0) { S[row * lds + b] = (uint8_t)e; }
+    }
+}
+
+// The transpose's form: a workgroup reads 128 rows of 32 columns into LDS and writes 32 rows of one block; 8 threads take a column,
+// 16 of its values each.
+constexpr int QT_COLS = 32;
+template <typename T>
+__global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size_t ldx, size_t rows, size_t cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, unsigned ncb)
+{
+    __shared__ float sh[ROWS_BLOCK][QT_COLS + 1];
+    const unsigned rb = blockIdx.x / ncb;
+    const size_t r0 = (size_t)rb * ROWS_BLOCK, c0 = (size_t)(blockIdx.x - rb * ncb) * QT_COLS;
+    for (int i = threadIdx.x; i < ROWS_BLOCK * QT_COLS; i += NT)
+    {
+        const int r = i / QT_COLS, c = i % QT_COLS;
+        sh[r][c] = r0 + r < rows && c0 + c < cols ? (float)X[(r0 + r) * ldx + c0 + c] : 0.0f;
+    }
+    __syncthreads();
+    const int c = threadIdx.x / 8, g = threadIdx.x % 8;
+    float x[16];
+    unsigned amax = 0u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { x[i] = sh[g * 16 + i][c]; amax = max(amax, finite_bits(x[i])); }
+    const unsigned e = block_exponent(lanes_max<8>(amax));
+    if (c0 + c >= cols) { return; }
+    const float f = block_factor(e);
+    uint8_t *q = Q + (c0 + c) * ldq + r0 + g * 16;
+    const size_t left = rows > r0 + g * 16 ? rows - (r0 + g * 16) : 0;
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { w[i] = pack_e4m3(x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f); }
+    if (left >= 16) { *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]); }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { if ((size_t)i < left) { q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4))); } }
+    }
+    if (g == 0) { S[(c0 + c) * lds + rb] = (uint8_t)e; }
+}
+
+// ---- launches ----
+// Threads a row and vectors a thread from the width alone: a row that fits 16 or 64 lanes needs no barrier; up to 1024 threads x 4
+// vectors hold a row (16 384 floats, 32 768 16-bit values), beyond that it is walked twice.
+#define ROWS_BY_WIDTH(T, cols, GO, WIDE)                                                                     \
+    do {                                                                                                     \
+        const int nv_ = ((cols) + vec_of<T>() - 1) / vec_of<T>();                                            \
+        if (nv_ <= 16) { GO(16, 1); }                                                                        \
+        else if (sizeof(T) == 4 && nv_ <= 32) { GO(16, 2); }                                                 \
+        else if (nv_ <= 64) { GO(64, 1); }                                                                   \
+        else if (nv_ <= 128) { GO(64, 2); }                                                                  \
+        else if (nv_ <= 256) { GO(64, 4); }                                                                  \
+        else if (nv_ <= 512) { GO(256, 2); }                                                                 \
+        else if (nv_ <= 1024) { GO(256, 4); }                                                                \
+        else if (nv_ <= 4096) { GO(1024, 4); }                                                               \
+        else { WIDE; }                                                                                       \
+    } while (0)
+
+constexpr size_t NORM_MAX_WG = 8192;
+
+template <typename T>
+void norm_go(const NormParams &p, hipStream_t s)
+{
+#define GO(TPR, CH)                                                                                          \
+    do {                                                                                                     \
+        constexpr int nth = TPR > NT ? TPR : NT, rpw = nth / TPR;                                            \
+        const size_t g = (p.rows + rpw - 1) / rpw;                                                           \
+        hipLaunchKernelGGL((norm_kernel<T, TPR, CH>), dim3((unsigned)(g < NORM_MAX_WG ? g : NORM_MAX_WG)), dim3(nth), 0, s, p); \
+    } while (0)
+    ROWS_BY_WIDTH(T, p.cols, GO, hipLaunchKernelGGL(norm_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p));
+#undef GO
+}
+
+template <typename T>
+void norm_grad_go(const NormGradParams &p, hipStream_t s)
+{
+    int groups = 0;
+#define GO(TPR, CH)                                                                                          \
+    do {                                                                                                     \
+        constexpr int nth = TPR > NT ? TPR : NT, rpw = nth / TPR;                                            \
+        const size_t g = (p.rows + rpw - 1) / rpw;                                                           \
+        groups = (int)(g < ROWS_GRAD_MAX_WG ? g : ROWS_GRAD_MAX_WG);                                         \
+        if (groups) { hipLaunchKernelGGL((norm_grad_kernel<T, TPR, CH>), dim3((unsigned)groups), dim3(nth), 0, s, p); } \
+    } while (0)
+#define WIDE                                                                                                 \
+    do {                                                                                                     \
+        groups = (int)(p.rows < 64 ? p.rows : 64);                                                           \
+        if (p.dW && groups) { hipLaunchKernelGGL(norm_grad_weight_kernel<T>, dim3((unsigned)((p.cols + NT - 1) / NT), (unsigned)groups), dim3(NT), 0, s, p, groups); } \
+        if (groups) { hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p); } \
+    } while (0)
+    ROWS_BY_WIDTH(T, p.cols, GO, WIDE);
+#undef WIDE
+#undef GO
+    if (p.dW) { hipLaunchKernelGGL(norm_grad_reduce_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(NT), 0, s, p.work, p.dW, p.cols, groups); }
+}
+
+template <typename T>
+void dropout_go(size_t rows, int cols, const void *X, size_t ldx, void *Y, size_t ldy, const DropParams &d, hipStream_t s)
+{
+    const int nv = (cols + vec_of<T>() - 1) / vec_of<T>();
+    const size_t total = rows * (size_t)nv, want = (total + NT - 1) / NT, grid = want < 4096 ? want : 4096, width = grid * NT;
+    hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)grid), dim3(NT), 0, s, reinterpret_cast<const T *>(X), reinterpret_cast<T *>(Y), ldx, ldy, rows, cols, nv,
+                       width / nv, (int)(width % nv), d);
+}
+
+template <typename T>
+void quantize_go(size_t rows, size_t cols, const void *X, size_t ldx, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, int transpose, hipStream_t s)
+{
+    const T *x = reinterpret_cast<const T *>(X);
+    if (transpose)
+    {
+        const size_t nrb = (rows + ROWS_BLOCK - 1) / ROWS_BLOCK, ncb = (cols + QT_COLS - 1) / QT_COLS;
+        hipLaunchKernelGGL(quantize_transpose_kernel<T>, dim3((unsigned)(nrb * ncb)), dim3(NT), 0, s, x, ldx, rows, cols, Q, ldq, S, lds, (unsigned)ncb);
+        return;
+    }
+    const size_t nb = (cols + ROWS_BLOCK - 1) / ROWS_BLOCK, want = (rows * nb + NT / 16 - 1) / (NT / 16);
+    hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)(want < 16384 ? want : 16384)), dim3(NT), 0, s, x, ldx, rows, cols, Q, ldq, S, lds, nb);
+}
+
+}  // namespace
+
+hipError_t launch_row_keys(const UttDesc *utts, uint32_t nutt, const TileDesc *tiles, uint32_t ntiles, int n, int offset,
+                           unsigned long long *base, unsigned long long *keys, hipStream_t s)
+{
+    hipLaunchKernelGGL(row_base_kernel, dim3(1), dim3(1024), 0, s, utts, nutt, n, offset, base);
+    hipLaunchKernelGGL(row_keys_kernel, dim3(ntiles), dim3(64), 0, s, tiles, n, offset, base, keys);
+    return hipGetLastError();
+}
+
+hipError_t launch_rows_dropout(int dtype, size_t rows, int cols, const void *X, size_t ldx, void *Y, size_t ldy, const DropParams &d, hipStream_t s)
+{
+    switch (dtype)
+    {
+        case SPEECH_F32: dropout_go<float>(rows, cols, X, ldx, Y, ldy, d, s); break;
+        case SPEECH_F64: dropout_go<double>(rows, cols, X, ldx, Y, ldy, d, s); break;
+        case SPEECH_BF16: dropout_go<__bf16>(rows, cols, X, ldx, Y, ldy, d, s); break;
+        case SPEECH_F16: dropout_go<_Float16>(rows, cols, X, ldx, Y, ldy, d, s); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_rows_norm(int dtype, const NormParams &p, hipStream_t s)
+{
+    switch (dtype)
+    {
+        case SPEECH_F32: norm_go<float>(p, s); break;
+        case SPEECH_BF16: norm_go<__bf16>(p, s); break;
+        case SPEECH_F16: norm_go<_Float16>(p, s); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_rows_norm_grad(int dtype, const NormGradParams &p, hipStream_t s)
+{
+    switch (dtype)
+    {
+        case SPEECH_F32: norm_grad_go<float>(p, s); break;
+        case SPEECH_BF16: norm_grad_go<__bf16>(p, s); break;
+        case SPEECH_F16: norm_grad_go<_Float16>(p, s); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_rows_quantize(int dtype, size_t rows, size_t cols, const void *X, size_t ldx, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds,
+                                int transpose, hipStream_t s)
+{
+    switch (dtype)
+    {
+        case SPEECH_F32: quantize_go<float>(rows, cols, X, ldx, Q, ldq, S, lds, transpose, s); break;
+        case SPEECH_BF16: quantize_go<__bf16>(rows, cols, X, ldx, Q, ldq, S, lds, transpose, s); break;
+        case SPEECH_F16: quantize_go<_Float16>(rows, cols, X, ldx, Q, ldq, S, lds, transpose, s); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace speech

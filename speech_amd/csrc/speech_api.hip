@@ -5,7 +5,7 @@
 // reference builds them per call (window c/kaldi_mfcc.c:105-135, mel c/kaldi_mfcc.c:157-188,
 // lifter c/kaldi_mfcc.c:200-210, equal loudness c/kaldi_plp.c:183-193), then kept on the device.
 // All arithmetic on audio happens in HIP kernels; there is no CPU fallback.
-#include "speech_internal.hpp"
+#include "rows_internal.hpp"
 #include "../../include/codee_speech.h"
 #include <cfloat>
 #include <cmath>
@@ -252,6 +252,7 @@ struct speech_batch {
     std::vector<unsigned long long> zrow;
     int zrow_n, zrow_off;
     int yoff_pow2;               // largest of 1, 2, 4 that divides every utterance's output offset (-1: not computed yet)
+    unsigned long long *d_krow;  // speech_batch_row_keys: first row of each utterance (allocated on first use)
     unsigned long long *d_ids;   // speech_batch_synth_audio: the utterances' corpus numbers (allocated on first use)
     unsigned long long max_n;    // longest utterance, samples
     unsigned long long max_w;    // longest utterance, frames
@@ -599,7 +600,7 @@ int speech::batch_fill(speech_batch *b, speech_plan *p, size_t nutt, const size_
                        const unsigned int *uids)
 {
     const char *fn = "speech_batch_create";
-    b->plan = p; b->d_utts = nullptr; b->d_tiles = nullptr; b->d_mom = nullptr; b->d_zrow = nullptr; b->zrow_n = b->zrow_off = -1; b->yoff_pow2 = -1; b->ev0 = b->ev1 = nullptr;
+    b->plan = p; b->d_utts = nullptr; b->d_tiles = nullptr; b->d_mom = nullptr; b->d_zrow = nullptr; b->d_krow = nullptr; b->zrow_n = b->zrow_off = -1; b->yoff_pow2 = -1; b->ev0 = b->ev1 = nullptr;
     b->d_ids = nullptr; b->max_n = 0; b->max_w = 0; b->d_plp_en = nullptr; b->plp_rows = 0;
     const bool plp_en = p->tuned && p->o.kind == SPEECH_PLP && p->o.use_energy;      // fast_mel.hip: energies travel between the two launches
     b->total_samples = b->total_out = b->total_frames = 0;
@@ -678,6 +679,7 @@ void speech_batch_destroy(speech_batch *b)
     if (b->d_mom) { (void)hipFree(b->d_mom); }
     if (b->d_plp_en) { (void)hipFree(b->d_plp_en); }
     if (b->d_zrow) { (void)hipFree(b->d_zrow); }
+    if (b->d_krow) { (void)hipFree(b->d_krow); }
     if (b->d_ids) { (void)hipFree(b->d_ids); }
     if (b->ev0) { (void)hipEventDestroy(b->ev0); }
     if (b->ev1) { (void)hipEventDestroy(b->ev1); }
@@ -923,6 +925,20 @@ int speech_batch_subsample_rows(const speech_batch *b, int n, int offset, size_t
         tot += r;
     }
     if (total_rows) { *total_rows = tot; }
+    return 0;
+}
+
+int speech_batch_row_keys(speech_batch *b, int n, int offset, unsigned long long *keys, void *stream)
+{
+    const char *fn = "speech_batch_row_keys";
+    if (!b || !b->plan) { return fail(fn, "null batch"); }
+    if (n < 1 || offset < 0 || offset >= n) { return fail(fn, "need n >= 1 and 0 <= offset < n"); }
+    if (b->tiles.empty()) { return 0; }
+    if (!keys) { return fail(fn, "null device pointer"); }
+    DeviceGuard g(b->plan->device);
+    if (!g.ok) { return fail(fn, "cannot select device %d", b->plan->device); }
+    if (!b->d_krow) { HIP_TRY(fn, hipMalloc((void **)&b->d_krow, b->utts.size() * sizeof(unsigned long long))); }
+    HIP_TRY(fn, launch_row_keys(b->d_utts, (uint32_t)b->utts.size(), b->d_tiles, (uint32_t)b->tiles.size(), n, offset, b->d_krow, keys, (hipStream_t)stream));
     return 0;
 }
 
