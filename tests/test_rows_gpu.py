@@ -412,20 +412,21 @@ def _unit(va, vb):
     """what the matrix unit may lose: it adds the products of 8 consecutive columns at a resolution of 2^-13 of the largest one's power
     of two, so each of the 7 others is off by less than 2^-13 of the largest: 7 2^-13 times the sum over groups of their largest
     magnitude (below, group by group; the largest is at most the product of the factors' largest)"""
-    m, n, k = len(va), len(vb), va.shape[1]
-    g = -(-k // 8)
-    pa, pb = np.zeros((m, g * 8)), np.zeros((n, g * 8))
-    pa[:, :k], pb[:, :k] = np.abs(va), np.abs(vb)
-    out = np.zeros((m, n))
+    torch = _t()
+    g = -(-va.shape[1] // 8)
+    pa, pb = (torch.nn.functional.pad(torch.from_numpy(np.abs(v)).cuda(), (0, g * 8 - v.shape[1])) for v in (va, vb))
+    out = torch.zeros(len(va), len(vb), dtype=torch.float64, device="cuda")
     for i in range(g):
-        a, b = pa[:, 8 * i:8 * i + 8], pb[:, 8 * i:8 * i + 8]
-        out += np.max([np.outer(a[:, j], b[:, j]) for j in range(8)], axis=0)
-    return 7 * 2.0 ** -13 * out
+        top = torch.zeros_like(out)
+        for j in range(8 * i, 8 * i + 8):
+            torch.maximum(top, pa[:, j, None] * pb[None, :, j], out=top)
+        out += top
+    return 7 * 2.0 ** -13 * out.cpu().numpy()
 
 
 PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 512, 2048), (2, 100, 130), (5, 33, 400), (16, 64, 1000), (17, 17, 17), (32, 257, 720), (98, 80, 257), (63, 130, 3000), (64, 512, 512),
             (130, 200, 385), (255, 256, 256), (257, 300, 129), (513, 129, 640), (998, 512, 720), (1, 4096, 33), (700, 1, 500), (3, 5, 0), (300, 1000, 1),
-            (1100, 1030, 900), (2048, 2560, 512)]
+            (1100, 1030, 900), (2048, 2560, 512), (4200, 2100, 300), (2817, 3333, 1152), (33000, 300, 128)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
