@@ -6,9 +6,15 @@
 // order and all 128 share their scale.  The unit adds the eight products of 8 bytes of a lane at a resolution of 2^-13 of the largest
 // (measured: beside 448 x 448 a product of 2^3 counts, one of 2^2 is lost), the rest in 32-bit floats.  Result: lane l holds column l & 15 (B's row), rows 4 (l >> 4) ... + 3.
 #include "rows_internal.hpp"
+#include <type_traits>
+#include <utility>
 
 namespace speech {
 namespace {
+
+// f(0), f(1), ... f(N - 1) as compile-time numbers
+template <typename FN, int... I> __device__ __forceinline__ void for_each_of(FN f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }
+template <int N, typename FN> __device__ __forceinline__ void for_each(FN f) { for_each_of(f, std::make_integer_sequence<int, N>()); }
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -121,10 +127,17 @@ __global__ __launch_bounds__(64 * WAVES) void product_split_kernel(const Product
 // banks; the loads write LDS in order and permute what they fetch instead.
 //
 // The unit gets B as its first operand, so that a lane's four results are four columns of one row of Y; which of a wave's rows of B sits at
-// which place of which 16-row tile is chosen so that all of a lane's columns are next to each other: 4 NN values, one or more 16-byte
-// stores.
+// which place of which 16-row tile is chosen so that two tiles give a lane eight columns next to each other, and four lanes 32: a 16-byte
+// store a lane, whole 64 bytes of a row.
+__device__ __forceinline__ void load_bias(const float *p, float (&v)[8])
+{
+    const VecOf<float, 4>::type x = *reinterpret_cast<const VecOf<float, 4>::type *>(p), y = *reinterpret_cast<const VecOf<float, 4>::type *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = x[i]; v[4 + i] = y[i]; }
+}
+
 __device__ __forceinline__ int swizzle_a(int row) { return row & 7; }
-template <int NN> __device__ __forceinline__ int swizzle_b(int row) { return (row & 3) | (((row / (4 * NN)) & 1) << 2); }
+__device__ __forceinline__ int swizzle_b(int row) { return (row & 3) | ((row >> 3 & 1) << 2); }
 
 // 16 bytes a lane from base + off into LDS at lds + 16 lane.  As an instruction of its own, because the compiler waits for every load
 // into LDS that it knows of before it reads any LDS; the waits are the caller's (vmcnt(0) before the barrier that publishes a
@@ -133,10 +146,20 @@ __device__ __forceinline__ void load_to_lds(const uint8_t *base, unsigned off, u
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
-// a dword a lane from its own address into LDS at lds + 4 lane
-__device__ __forceinline__ void load_dword_to_lds(const uint8_t *from, unsigned lds)
+// the same with the place as lds + STEP, in one scalar instruction
+template <int STEP>
+__device__ __forceinline__ void load_to_lds_at(const uint8_t *base, unsigned off, unsigned lds)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(from) : "memory", "m0");
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base), "n"(STEP) : "memory", "m0", "scc");
+}
+// a dword a lane from each of two arrays into LDS at lds + 4 lane and 1024 behind, or nothing, without a branch: the loads of no lane
+__device__ __forceinline__ void load_dwords_to_lds_if(bool yes, const uint8_t *one, unsigned off1, const uint8_t *two, unsigned off2, unsigned lds)
+{
+    unsigned long long all;
+    const int lanes = __builtin_amdgcn_readfirstlane(yes ? -1 : 0);
+    asm volatile("s_mov_b64 %0, exec\n\ts_mov_b32 exec_lo, %1\n\ts_mov_b32 exec_hi, %1\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %3, %4\n\t"
+                 "s_add_u32 m0, %2, 0x400\n\ts_nop 0\n\tglobal_load_lds_dword %5, %6\n\ts_mov_b64 exec, %0"
+                 : "=&s"(all) : "s"(lanes), "s"(lds), "v"(off1), "s"(one), "v"(off2), "s"(two) : "memory", "m0", "scc");
 }
 
 template <typename T, int TM, int TN, int WM, int WN>
@@ -171,7 +194,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
     for (int i = 0; i < LB; ++i)
     {
         const int row = i * (NTH / 8) + tid / 8;
-        ob[i] = (unsigned)min(row, bm) * ldb + (unsigned)(((tid & 7) ^ swizzle_b<NN>(row)) * 16);
+        ob[i] = (unsigned)min(row, bm) * ldb + (unsigned)(((tid & 7) ^ swizzle_b(row)) * 16);
     }
     const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds + (unsigned)wave * 1024u);
     const int last = (int)(p.K - (size_t)(nb - 1) * 128);                    // bytes of the last k-step: 1 ... 128
@@ -192,7 +215,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
 #pragma unroll
         for (int i = 0; i < LB; ++i)
         {
-            const int row = i * (NTH / 8) + tid / 8, c = (tid & 7) ^ swizzle_b<NN>(row);
+            const int row = i * (NTH / 8) + tid / 8, c = (tid & 7) ^ swizzle_b(row);
             const unsigned o = cut && c * 16 >= last ? ob[i] - (unsigned)(c * 16) : ob[i];
             load_to_lds(B + k, o, dst + (unsigned)(TM * 128 + i * (NTH * 16)));
         }
@@ -204,7 +227,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
 #pragma unroll
     for (int i = 0; i < MT; ++i) { SA[i] = p.SA + (m0 + (size_t)min(wm * (TM / WM) + 16 * i + l16, am)) * p.ldsa; }
 #pragma unroll
-    for (int j = 0; j < NN; ++j) { SB[j] = p.SB + (n0 + (size_t)min(wn * (TN / WN) + 4 * NN * (l16 >> 2) + 4 * j + (l16 & 3), bm)) * p.ldsb; }
+    for (int j = 0; j < NN; ++j) { SB[j] = p.SB + (n0 + (size_t)min(wn * (TN / WN) + 32 * (j >> 1) + 4 * (j & 1) + 8 * (l16 >> 2) + (l16 & 3), bm)) * p.ldsb; }
     auto fetch_scales = [&](int kb)
     {
 #pragma unroll
@@ -238,7 +261,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
         {
             for (int r = tid; r < TM + TN; r += NTH)
             {
-                const int f = r < TM ? swizzle_a(r) : swizzle_b<NN>(r - TM);
+                const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
                 for (int c = last / 16; c < 8; ++c)
                 {
                     uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
@@ -256,9 +279,9 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
 #pragma unroll
         for (int j = 0; j < NN; ++j)
         {
-            const int row = wn * (TN / WN) + 4 * NN * (l16 >> 2) + 4 * j + (l16 & 3);
+            const int row = wn * (TN / WN) + 32 * (j >> 1) + 4 * (j & 1) + 8 * (l16 >> 2) + (l16 & 3);
             const uint8_t *q = st + TM * 128 + row * 128;
-            const int c = g ^ swizzle_b<NN>(row);
+            const int c = g ^ swizzle_b(row);
             const int4 x = *reinterpret_cast<const int4 *>(q + c * 16), y = *reinterpret_cast<const int4 *>(q + (c ^ 4) * 16);
             fb[j] = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
         }
@@ -279,209 +302,261 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
         for (int j = 0; j < NN; ++j) { sb[j] >>= 8; }
     }
 
-    const size_t n = n0 + (size_t)(wn * (TN / WN) + 4 * NN * g);
-    const int left = n < p.N ? (int)min(p.N - n, (size_t)(4 * NN)) : 0;
-    float bias[4 * NN];
+    const size_t n = n0 + (size_t)(wn * (TN / WN) + 8 * g);
 #pragma unroll
-    for (int q = 0; q < 4 * NN; ++q) { bias[q] = p.bias && q < left ? p.bias[n + q] : 0.0f; }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int h = 0; h < NN / 2; ++h)
     {
-        const size_t m = m0 + (size_t)(wm * (TM / WM) + 16 * i + l16);
-        if (m >= p.M) { continue; }
-        T *y = reinterpret_cast<T *>(p.Y) + m * p.ldy + n;
+        const int left = n + 32 * h < p.N ? (int)min(p.N - (n + 32 * h), (size_t)8) : 0;
+        float bias[8];
 #pragma unroll
-        for (int h = 0; h < 4 * NN; h += 8)
+        for (int q = 0; q < 8; ++q) { bias[q] = p.bias && q < left ? p.bias[n + 32 * h + q] : 0.0f; }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
         {
+            const size_t m = m0 + (size_t)(wm * (TM / WM) + 16 * i + l16);
             float v[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) { v[q] = acc[i][(h + q) / 4][q % 4] + bias[h + q]; }
-            store_vals(y + h, left - h, v);
+            for (int q = 0; q < 8; ++q) { v[q] = acc[i][2 * h + q / 4][q % 4] + bias[q]; }
+            if (m < p.M) { store_vals(reinterpret_cast<T *>(p.Y) + m * p.ldy + n + 32 * h, left, v); }
         }
     }
 }
 
-// ---- the largest products: two groups of waves in turn ----
-// 256 x 256 values, 8 waves of 128 x 64.  A SIMD holds one wave of each group; time runs in phases between barriers, and in each phase one
-// group reads its operands of a k-step from LDS into registers while the other one's 32 matrix instructions run, so that neither the
-// matrix unit nor LDS waits for the other:
+// ---- the largest products: one wave a SIMD, one stream of k-steps over all tiles ----
+// 256 x 256 values, 4 waves of 128 x 128: the fewest operand bytes out of LDS for a value (128 + 128 rows feed 128 x 128), and one
+// instruction stream that never has to wait between its matrix instructions.  256 sums, 128 registers of operands, 16 of scales.
 //
-//   phase 2 s      group 0 reads step s          group 1 computes step s - 1      all ask for stage s + 1
-//   phase 2 s + 1  group 0 computes step s       group 1 reads step s             at its end stage s + 1 is there
+// A k-step is 64 matrix instructions.  The first 32 take rows 0 ... 63 of the wave's A, the others rows 64 ... 127, each time column tile by
+// column tile; an operand's registers are filled for the next use as soon as the last instruction that reads them has been issued:
 //
-// Stage s + 1 takes the buffer of stage s - 1, which group 1 read in phase 2 s - 1.  Scales go through LDS as well, four k-steps (a dword
-// a row) at a time.
+//   first half    A's second half is read from this step's stage at once
+//   barrier       after a quarter of it: all waves have read this stage; from here on the loads of the stage after the next, which takes its
+//                 place, go out one by one between the matrix instructions
+//   barrier       in the middle: all waves have seen the next stage arrive
+//   second half   A's first half and, column tile by column tile as they fall free, B are read from the next stage
 //
-// 128 sums, 96 registers of operands and 12 of scales leave 20 for everything else: a wave's LDS addresses differ by constants only, and
-// the last tiles of rows and columns are moved back to end with the matrix, so that no tile has an edge (what two tiles share they compute
-// alike).  M and N are at least 256.
-template <typename T>
-__global__ __launch_bounds__(512) void product_turn_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
+// So a load has between one and one and a half k-steps of 2048 matrix cycles to arrive.  A CU takes 64 bytes a cycle into LDS (measured),
+// a stage of 64 KB occupies it for half of a k-step; a load that finds the queue full holds up everything behind it, hence one by
+// one.
+//
+// A workgroup stays on its CU and walks tiles; the stages of its next tile follow those of this one without a gap, so that only the
+// writing of the results stands between two tiles.  The last tiles of rows and columns are moved back to end with the matrix, so that no
+// tile has an edge (what two tiles share they compute alike).  M and N are at least 256, K more than 384 (four k-steps).
+// TAIL: K is no multiple of 128.
+template <typename T, bool TAIL>
+__global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
 {
-    constexpr int TM = 256, TN = 256, MT = 8, NN = 4, STAGE = (TM + TN) * 128, SCALES = 2 * STAGE;
+    constexpr int TM = 256, TN = 256, MT = 8, NN = 8, STAGE = (TM + TN) * 128, SCALES = 2 * STAGE;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, l16 = tid & 15, g = (tid >> 4) & 3;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = wave >> 2, wn = wave & 3;
-
-    const unsigned total = tiles_m * tiles_n, per = (total + 7) / 8;
-    const unsigned tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (tile >= total) { return; }
-    const unsigned band = tile / (8 * tiles_n), in = tile - band * 8 * tiles_n, bh = min(8u, tiles_m - band * 8);
-    const size_t m0 = min((size_t)(band * 8 + in % bh) * TM, p.M - TM), n0 = min((size_t)(in / bh) * TN, p.N - TN);
-
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
     const int nb = (int)((p.K + 127) / 128), last = (int)(p.K - (size_t)(nb - 1) * 128);
-    const uint8_t *A = p.A + m0 * p.lda, *B = p.B + n0 * p.ldb;
-    // a load brings 64 rows, 8 a wave: thread t takes the chunk of row t / 8 that belongs at place t % 8
-    const int lr = tid >> 3, ca = (tid & 7) ^ swizzle_a(lr), cb = (tid & 7) ^ swizzle_b<NN>(lr);
-    const unsigned oa = (unsigned)lr * (unsigned)p.lda + (unsigned)(ca * 16), ob = (unsigned)lr * (unsigned)p.ldb + (unsigned)(cb * 16);
-    const uint8_t *S = tid < TM ? p.SA + (m0 + tid) * p.ldsa : p.SB + (n0 + tid - TM) * p.ldsb;
-    const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    const unsigned lds0 = __builtin_amdgcn_readfirstlane(base) + (unsigned)wave * 1024u, sc0 = __builtin_amdgcn_readfirstlane(base) + SCALES + (unsigned)wave * 256u;
 
-    // chunks that start at or behind K are fetched from the row's first bytes (clear() zeroes them)
-    auto fetch = [&](int kb)
+    // XCDs take workgroups in turn: each gets a run of consecutive tiles, which walk 8 tiles of rows at a time so that the 32 tiles an XCD
+    // works on share their rows of A and B in its L2
+    const unsigned total = tiles_m * tiles_n, per = (total + 7) / 8, first = (blockIdx.x & 7) * per, end = min(first + per, total), stride = gridDim.x >> 3;
+    unsigned tile = first + (blockIdx.x >> 3);
+    if (tile >= end) { return; }
+    auto corner = [&](unsigned t, size_t &m0, size_t &n0)
     {
-        if (kb >= nb) { return; }
-        unsigned fa = oa, fb = ob;
-        if (kb == nb - 1 && last < 128)
-        {
-            if (ca * 16 >= last) { fa -= (unsigned)(ca * 16); }
-            if (cb * 16 >= last) { fb -= (unsigned)(cb * 16); }
-        }
-        const uint8_t *a = A + (size_t)kb * 128, *b = B + (size_t)kb * 128;
-        const unsigned dst = lds0 + (unsigned)((kb & 1) * STAGE);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { load_to_lds(a + (size_t)i * 64 * p.lda, fa, dst + (unsigned)(i * 8192)); }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { load_to_lds(b + (size_t)i * 64 * p.ldb, fb, dst + (unsigned)(TM * 128 + i * 8192)); }
-        if ((kb & 3) == 0) { load_dword_to_lds(S + kb, sc0 + (unsigned)((kb >> 2 & 1) * 2048)); }
+        const unsigned band = t / (8 * tiles_n), in = t - band * 8 * tiles_n, bh = min(8u, tiles_m - band * 8);
+        m0 = min((size_t)(band * 8 + in % bh) * TM, p.M - TM);
+        n0 = min((size_t)(in / bh) * TN, p.N - TN);
     };
+
+    // a load brings 32 rows, 8 a wave: thread t takes the chunk of row t / 8 that belongs at place t % 8
+    const int lr = tid >> 3, ca = (tid & 7) ^ swizzle_a(lr), cb = (tid & 7) ^ swizzle_b(lr);
+    const unsigned stepa = 32u * (unsigned)p.lda, stepb = 32u * (unsigned)p.ldb;
+    const unsigned oa = (unsigned)lr * (unsigned)p.lda + (unsigned)(ca * 16), ob = (unsigned)lr * (unsigned)p.ldb + (unsigned)(cb * 16);
+    const unsigned osa = (unsigned)tid * (unsigned)p.ldsa, osb = (unsigned)tid * (unsigned)p.ldsb;
+    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds);
+    const unsigned lds0 = base + (unsigned)wave * 1024u, sc0 = base + SCALES + (unsigned)wave * 256u;
+
+    // what is being fetched: the k-step at A, B of a tile whose scales start at SA, SB
+    const uint8_t *A, *B, *SA, *SB;
+    unsigned fstage = 0, fscales = 0;
+    auto fetch = [&](auto i, unsigned fa, unsigned fb)                       // the i-th of a stage's 16 loads
+    {
+        constexpr int I = decltype(i)::value;
+        if (I < 8) { load_to_lds_at<I * 4096>(A, fa + I * stepa, lds0 + fstage); }
+        else { load_to_lds_at<I * 4096>(B, fb + (I - 8) * stepb, lds0 + fstage); }
+    };
+    auto fetch_scales = [&](int fk, bool yes)                                // of k-steps fk ... fk + 3, or nothing
+    {
+        load_dwords_to_lds_if(yes, SA + fk, osa, SB + fk, osb, sc0 + fscales);
+        fscales ^= yes ? 2048u : 0u;
+    };
+    auto wait_read = []() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); };
     auto barrier = []()
     {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_barrier" : : : "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // group 0, at the start of the phase in which it reads the last stage
-    auto clear = [&]()
-    {
-        uint8_t *st = lds + ((nb - 1) & 1) * STAGE;
-        for (int r = tid; r < TM + TN; r += 256)
-        {
-            const int f = r < TM ? swizzle_a(r) : swizzle_b<NN>(r - TM);
-            for (int c = last / 16; c < 8; ++c)
-            {
-                uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
-                *q = keep_bytes(*q, last - c * 16);
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    };
 
     v4f acc[MT][NN];
     v8i fa[MT], fb[NN];
     int sa[MT], sb[NN];
+    // row 16 i + l16 of A: chunk g ^ (l16 & 7); row 32 (j / 2) + 4 (j % 2) + 8 (l16 / 4) + l16 % 4 of B: the same
+    const int place = (g ^ (l16 & 7)) * 16, brow = wn * 128 + 8 * (l16 >> 2) + (l16 & 3), arow = wm * 128 + l16;
+    const int qa = arow * 128 + place, qb = TM * 128 + brow * 128 + place, qsa = SCALES + arow * 4, qsb = SCALES + (TM + brow) * 4;
+    unsigned stage = 0, scales = 0;                                          // of the step that is read; scales: its byte among four as well
+    auto read_a = [&](int i)
+    {
+        const uint8_t *q = lds + stage;
+        const int4 x = *reinterpret_cast<const int4 *>(q + qa + i * 2048), y = *reinterpret_cast<const int4 *>(q + (qa ^ 64) + i * 2048);
+        fa[i] = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        sa[i] = lds[scales + qsa + i * 64];
+    };
+    auto read_b = [&](int j)
+    {
+        const uint8_t *q = lds + stage;
+        const int o = (j >> 1) * 4096 + (j & 1) * 512;
+        const int4 x = *reinterpret_cast<const int4 *>(q + qb + o), y = *reinterpret_cast<const int4 *>(q + (qb ^ 64) + o);
+        fb[j] = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        sb[j] = lds[scales + qsb + (j >> 1) * 128 + (j & 1) * 16];
+    };
+
+    // The next tile's operands, found when this one begins; behind the last tile its own once more: what is fetched then nobody reads.
+    size_t m0, n0, mx, nx;
+    const uint8_t *nA, *nB, *nSA, *nSB;
+    auto look_ahead = [&]()
+    {
+        corner(tile + stride < end ? tile + stride : tile, mx, nx);
+        nA = p.A + mx * p.lda; nB = p.B + nx * p.ldb; nSA = p.SA + mx * p.ldsa; nSB = p.SB + nx * p.ldsb;
+    };
+    corner(tile, m0, n0);
+    A = p.A + m0 * p.lda; B = p.B + n0 * p.ldb; SA = p.SA + m0 * p.ldsa; SB = p.SB + n0 * p.ldsb;
+    fetch_scales(0, true);
+    for_each<16>([&](auto i) { fetch(i, oa, ob); });
+    fstage ^= (unsigned)STAGE;
+    A += 128; B += 128;
+    for_each<16>([&](auto i) { fetch(i, oa, ob); });
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    barrier();
+#pragma unroll
+    for (int j = 0; j < NN; ++j) { read_b(j); }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { read_a(i); }
+    look_ahead();
 #pragma unroll
     for (int i = 0; i < MT; ++i)
     {
 #pragma unroll
         for (int j = 0; j < NN; ++j) { acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f}; }
     }
-    // row 16 i + l16 of A: chunk g ^ (row & 7); row 16 (l16 / 4) + 4 j + l16 % 4 of B: chunk g ^ (l16 % 4 + 4 (l16 / 4 % 2)) = g ^ (l16 & 7)
-    const int place = (g ^ (l16 & 7)) * 16, brow = wn * 64 + 16 * (l16 >> 2) + (l16 & 3), arow = group * 128 + l16;
-    const int qa = arow * 128 + place, qb = TM * 128 + brow * 128 + place, qsa = SCALES + arow * 4, qsb = SCALES + (TM + brow) * 4;
-    auto read = [&](int kb)
-    {
-        const uint8_t *st = lds + (kb & 1) * STAGE, *sc = lds + ((kb >> 2 & 1) * 2048 + (kb & 3));
-        const uint8_t *a0 = st + qa, *a1 = st + (qa ^ 64), *b0 = st + qb, *b1 = st + (qb ^ 64);
-#pragma unroll
-        for (int j = 0; j < NN; ++j)
-        {
-            const int4 x = *reinterpret_cast<const int4 *>(b0 + j * 512), y = *reinterpret_cast<const int4 *>(b1 + j * 512);
-            fb[j] = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-            sb[j] = sc[qsb + j * 16];
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-        {
-            const int4 x = *reinterpret_cast<const int4 *>(a0 + i * 2048), y = *reinterpret_cast<const int4 *>(a1 + i * 2048);
-            fa[i] = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-            sa[i] = sc[qsa + i * 64];
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-    };
-    auto compute = [&]()
-    {
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-        {
-#pragma unroll
-            for (int j = 0; j < NN; ++j) { acc[i][j] = mfma_scaled(fb[j], fa[i], acc[i][j], sb[j], sa[i]); }
-        }
-        __builtin_amdgcn_s_setprio(0);
-    };
 
-    fetch(0);
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    barrier();
-    if (group == 0)
+    // Between two matrix instructions there is room for the issue of about six others: what else a step has to do is handed out to its 2 x
+    // 32 places, and kept there; without TAIL a step is one run of instructions without a branch, across which the compiler would move
+    // them.  Place m of a half: column tile m / 4, row tile m % 4 (+ 4).
+    auto multiply = [&](int i, int j)
     {
-        for (int kb = 0; kb < nb; ++kb)
-        {
-            if (kb == nb - 1 && last < 128) { clear(); barrier(); }
-            fetch(kb + 1);
-            read(kb);
-            barrier();
-            compute();
-            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-            barrier();
-        }
-    }
-    else
+        acc[i][j] = mfma_scaled(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    for (;;)
     {
-        for (int kb = -1; kb < nb; ++kb)
+        for (int k = 0; k < nb; ++k)                                         // k-step k + 2 is asked for, which for the last two is the next tile's
         {
-            if (kb >= 0)
+            unsigned fo = oa, go = ob;
+            for_each<32>([&](auto mm)
             {
-                read(kb);
-                asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-                barrier();
+                constexpr int m = decltype(mm)::value;
+                if (m < 4) { read_a(4 + m); }
+                if (m == 8)
+                {
+                    wait_read();
+                    barrier();                                                   // all have read this stage
+                    fstage ^= (unsigned)STAGE;
+                    const bool next = k == nb - 2;
+                    A = next ? nA : A + 128; B = next ? nB : B + 128;
+                    if (TAIL)                                                    // chunks that start at or behind K come from the row's first bytes
+                    {
+                        fo -= k == nb - 3 && ca * 16 >= last ? (unsigned)(ca * 16) : 0u;
+                        go -= k == nb - 3 && cb * 16 >= last ? (unsigned)(cb * 16) : 0u;
+                    }
+                }
+                if (m == 12)
+                {
+                    const bool next = k == nb - 2;
+                    SA = next ? nSA : SA; SB = next ? nSB : SB;
+                    fetch_scales(next ? 0 : k + 2, next || ((k & 3) == 2 && k < nb - 2));
+                }
+                if constexpr (m >= 9 && m % 4 == 1) { fetch(std::integral_constant<int, (m - 9) / 4>(), fo, go); }
+                multiply(m % 4, m / 4);
+            });
+            asm volatile("s_waitcnt vmcnt(6)" : : : "memory");                   // all but the six loads above
+            barrier();                                                           // the next stage is there
+            stage ^= (unsigned)STAGE;
+            // the next step's scale byte; behind a group of four or the tile, the other buffer's first
+            scales = k == nb - 1 || (k & 3) == 3 ? (scales & 2048u) ^ 2048u : scales + 1u;
+            if (TAIL)
+            {
+                if (k == nb - 2)
+                {
+                    uint8_t *st = lds + stage;
+                    for (int r = tid; r < TM + TN; r += 256)
+                    {
+                        const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
+                        for (int c = last / 16; c < 8; ++c)
+                        {
+                            uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
+                            *q = keep_bytes(*q, last - c * 16);
+                        }
+                    }
+                    wait_read();
+                    barrier();
+                }
             }
-            if (kb == nb - 2 && last < 128) { barrier(); }
-            fetch(kb + 2);
-            if (kb >= 0) { compute(); }
-            if (kb < nb - 1) { barrier(); }
+            for_each<32>([&](auto mm)
+            {
+                constexpr int m = decltype(mm)::value;
+                if (m % 2 == 1 && m < 8) { read_a(m / 2); }
+                if (m % 4 == 0 && m > 0) { read_b(m / 4 - 1); }
+                if constexpr (m % 4 == 2) { fetch(std::integral_constant<int, 6 + m / 4>(), fo, go); }
+                if constexpr (m == 11 || m == 19) { fetch(std::integral_constant<int, m == 11 ? 14 : 15>(), fo, go); }
+                multiply(4 + m % 4, m / 4);
+            });
+            read_b(7);
+            __builtin_amdgcn_sched_barrier(0);
         }
-    }
-
-    const size_t n = n0 + (size_t)(wn * 64 + 16 * g);
-    float bias[16];
+        // rows after rows from one address: a table of them, kept over the tiles, would push out the operands
+        size_t ldy = p.ldy;
+        int row = arow, col = wn * 128 + 8 * g;
+        asm volatile("" : "+s"(ldy), "+v"(row), "+v"(col));
+        const size_t n = n0 + (size_t)col;
 #pragma unroll
-    for (int q = 0; q < 16; ++q) { bias[q] = p.bias ? p.bias[n + q] : 0.0f; }
-    T *y = reinterpret_cast<T *>(p.Y) + (m0 + (size_t)arow) * p.ldy + n;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-    {
-#pragma unroll
-        for (int h = 0; h < 16; h += 8)
+        for (int h = 0; h < NN / 2; ++h)
         {
-            float v[8];
+            T *y = reinterpret_cast<T *>(p.Y) + (m0 + (size_t)row) * ldy + n + 32 * h;
+            float bias[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (p.bias) { load_bias(p.bias + n + 32 * h, bias); }
 #pragma unroll
-            for (int q = 0; q < 8; ++q) { v[q] = acc[i][(h + q) / 4][q % 4] + bias[h + q]; }
-            store_vals(y + (size_t)(16 * i) * p.ldy + h, 8, v);
+            for (int i = 0; i < MT; ++i)
+            {
+                float v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { v[q] = acc[i][2 * h + q / 4][q % 4] + bias[q]; acc[i][2 * h + q / 4][q % 4] = 0.0f; }
+                store_vals(y, 8, v);
+                y += 16 * ldy;
+            }
         }
+        tile += stride;
+        if (tile >= end) { break; }
+        m0 = mx; n0 = nx;
+        look_ahead();
     }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");                       // the loads behind the last tile, before its LDS is another's
 }
 
-template <typename T>
-hipError_t turn_go(const ProductParams &p, hipStream_t s)
+template <typename T, bool TAIL>
+hipError_t stream_go(const ProductParams &p, hipStream_t s)
 {
     constexpr int LDS = 2 * 512 * 128 + 2 * 2048;
-    const hipError_t e = opt_in_lds_once(reinterpret_cast<const void *>(&product_turn_kernel<T>), LDS);
+    const hipError_t e = opt_in_lds_once(reinterpret_cast<const void *>(&product_stream_kernel<T, TAIL>), LDS);
     if (e != hipSuccess) { return e; }
-    const unsigned tm = (unsigned)((p.M + 255) / 256), tn = (unsigned)((p.N + 255) / 256);
-    hipLaunchKernelGGL(product_turn_kernel<T>, dim3((tm * tn + 7) / 8 * 8), dim3(512), LDS, s, p, tm, tn);
+    const unsigned tm = (unsigned)((p.M + 255) / 256), tn = (unsigned)((p.N + 255) / 256), want = (tm * tn + 7) / 8 * 8;
+    hipLaunchKernelGGL((product_stream_kernel<T, TAIL>), dim3(want < 256u ? want : 256u), dim3(256), LDS, s, p, tm, tn);
     return hipSuccess;
 }
 
@@ -501,8 +576,8 @@ template <typename T>
 hipError_t product_go(const ProductParams &p, hipStream_t s)
 {
     // rows of a tile are addressed in 32 bits from its first
-    const bool near = p.lda < ((size_t)1 << 23) && p.ldb < ((size_t)1 << 23);
-    if (near && p.M >= 256 && p.N >= 256 && p.K > 0 && ((p.M + 255) / 256) * ((p.N + 255) / 256) >= 128) { return turn_go<T>(p, s); }
+    const bool near = p.lda < ((size_t)1 << 23) && p.ldb < ((size_t)1 << 23) && p.ldsa < ((size_t)1 << 23) && p.ldsb < ((size_t)1 << 23);
+    if (near && p.M >= 256 && p.N >= 256 && p.K > 384 && ((p.M + 255) / 256) * ((p.N + 255) / 256) >= 128) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
     if (near && ((p.M + 127) / 128) * ((p.N + 127) / 128) >= 64) { return tile_go<T, 128, 128, 2, 2>(p, s); }
     const size_t tm = (p.M + 31) / 32, tn = (p.N + 31) / 32;
     hipLaunchKernelGGL((product_split_kernel<T, 2, 2, 4>), dim3((unsigned)(tm * tn)), dim3(256), 0, s, p, (unsigned)tn);
