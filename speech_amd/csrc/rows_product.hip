@@ -485,7 +485,9 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
                 if constexpr (m >= 9 && m % 4 == 1) { fetch(std::integral_constant<int, (m - 9) / 4>(), fo, go); }
                 multiply(m % 4, m / 4);
             });
-            asm volatile("s_waitcnt vmcnt(6)" : : : "memory");                   // all but the six loads above
+            // all but the six loads above and, in a tile's first step, the 32 stores of the tile before (memory instructions are counted off in
+            // the order of their issue); the choice stands inside the asm, because a branch would end the run of instructions
+            asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(6)\n\ts_branch 2f\n1:\ts_waitcnt vmcnt(38)\n2:" : : "s"(k) : "memory", "scc");
             barrier();                                                           // the next stage is there
             stage ^= (unsigned)STAGE;
             // the next step's scale byte; behind a group of four or the tile, the other buffer's first
