@@ -151,6 +151,54 @@ __device__ __forceinline__ void norm_input(const NormParams &p, size_t row, int 
     for (int i = 0; i < N; ++i) { h[i] = (float)(T)h[i]; }
 }
 
+// The same for CH vectors of a row, all loads before the first use; 0 behind the row's end.
+template <typename T, int TPR, int CH, int N>
+__device__ __forceinline__ void norm_inputs(const NormParams &p, size_t row, int t, unsigned long long fk, float (&h)[CH][N])
+{
+    const T *X = reinterpret_cast<const T *>(p.X) + row * p.ldx, *R = reinterpret_cast<const T *>(p.R) + row * p.ldr;
+    float r[CH][N];
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+    {
+        const int c = (k * TPR + t) * N;
+        load_vals<float>(X + c, p.cols - c, h[k]);
+    }
+    if (p.R)
+    {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+            const int c = (k * TPR + t) * N;
+            load_vals<float>(R + c, p.cols - c, r[k]);
+        }
+    }
+    if (p.drop.on)
+    {
+        const float scale = (float)p.drop.scale;
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i) { h[k][i] = drop_keeps(fk, (unsigned)((k * TPR + t) * N + i), p.drop.thresh) ? h[k][i] * scale : 0.0f; }
+        }
+    }
+    if (p.R)
+    {
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+#pragma unroll
+            for (int i = 0; i < N; ++i) { h[k][i] += r[k][i]; }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { h[k][i] = (float)(T)h[k][i]; }
+    }
+}
+
 __device__ __forceinline__ float rstd_of(float ss, const NormParams &p) { return 1.0f / sqrtf(ss / (float)p.cols + p.eps); }
 
 template <int N>
@@ -171,7 +219,8 @@ __device__ __forceinline__ void store_e4m3(uint8_t *q, int n, const float (&y)[N
     }
 }
 
-// A row stays in the registers of its TPR threads, CH vectors each, from its one reading to its one writing.
+// A row stays in the registers of its TPR threads, CH vectors each, from its one reading to its one writing; the weight's vectors stay
+// there for all of a thread's rows.
 template <typename T, int TPR, int CH>
 __global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormParams p)
 {
@@ -181,18 +230,24 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormPar
     int flip = 0;
     const unsigned long long ku = drop_layer_key(p.drop);
     const int nb = (p.cols + ROWS_BLOCK - 1) / ROWS_BLOCK;
+    constexpr bool HOLD = TPR < 1024;                                        // 1024 threads have 128 registers each
+    float w[CH][N];
+    if (HOLD)
+    {
+#pragma unroll
+        for (int k = 0; k < CH; ++k) { load_weight<T>(p.weight, p.weight_f32, (k * TPR + t) * N, p.cols - (k * TPR + t) * N, w[k]); }
+    }
     for (size_t row = (size_t)blockIdx.x * RPW + threadIdx.x / TPR; row < p.rows; row += (size_t)gridDim.x * RPW)
     {
         const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
         float h[CH][N];
+        norm_inputs<T, TPR>(p, row, t, fk, h);
         float ss = 0.0f;
 #pragma unroll
         for (int k = 0; k < CH; ++k)
         {
-            const int c = (k * TPR + t) * N;
-            norm_input<T>(p, row, c, fk, h[k]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) { ss += c + i < p.cols ? h[k][i] * h[k][i] : 0.0f; }
+            for (int i = 0; i < N; ++i) { ss += h[k][i] * h[k][i]; }        // 0 behind the row
         }
         if (p.H)
         {
@@ -209,10 +264,9 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormPar
         for (int k = 0; k < CH; ++k)
         {
             const int c = (k * TPR + t) * N;
-            float w[N];
-            load_weight<T>(p.weight, p.weight_f32, c, p.cols - c, w);
+            if (!HOLD) { load_weight<T>(p.weight, p.weight_f32, c, p.cols - c, w[k]); }
 #pragma unroll
-            for (int i = 0; i < N; ++i) { h[k][i] = h[k][i] * rstd * w[i]; }
+            for (int i = 0; i < N; ++i) { h[k][i] = h[k][i] * rstd * w[k][i]; }
             if (p.Y) { store_vals(reinterpret_cast<T *>(p.Y) + row * p.ldy + c, p.cols - c, h[k]); }
         }
         if (p.Q)
@@ -223,7 +277,7 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormPar
             {
                 amax[k] = 0u;
 #pragma unroll
-                for (int i = 0; i < N; ++i) { amax[k] = max(amax[k], (k * TPR + t) * N + i < p.cols ? finite_bits(h[k][i]) : 0u); }
+                for (int i = 0; i < N; ++i) { amax[k] = max(amax[k], finite_bits(h[k][i])); }
             }
             if (TPR < LB)                                                    // the whole row is one block
             {
@@ -295,7 +349,7 @@ __global__ __launch_bounds__(NT) void norm_wide_kernel(const NormParams p)
 }
 
 // ---- backward ----
-// g = dY w of N elements; returns dY h summed with the weight: what the row's mean takes
+// g = dY w of N elements; returns their sum of g h
 template <typename T, int N>
 __device__ __forceinline__ float grad_input(const NormGradParams &p, size_t row, int c, float (&dy)[N], float (&h)[N], float (&g)[N])
 {
@@ -309,19 +363,11 @@ __device__ __forceinline__ float grad_input(const NormGradParams &p, size_t row,
     return s;
 }
 
+// dh in 32 bits to dH, and through the mask to dX
 template <typename T, int N>
-__device__ __forceinline__ void grad_output(const NormGradParams &p, size_t row, int c, unsigned long long fk, float rstd, float coef, const float (&h)[N], float (&g)[N])
+__device__ __forceinline__ void grad_store(const NormGradParams &p, size_t row, int c, unsigned long long fk, float (&g)[N])
 {
     const int n = p.cols - c;
-#pragma unroll
-    for (int i = 0; i < N; ++i) { g[i] = g[i] * rstd - h[i] * coef; }
-    if (p.dR)
-    {
-        float r[N];
-        load_vals<float>(reinterpret_cast<const T *>(p.dR) + row * p.lddr + c, n, r);
-#pragma unroll
-        for (int i = 0; i < N; ++i) { g[i] += r[i]; }
-    }
     if (p.dH) { store_vals(reinterpret_cast<T *>(p.dH) + row * p.lddh + c, n, g); }
     if (p.dX)
     {
@@ -357,20 +403,39 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_grad_kernel(const No
     {
         const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
         const float rstd = p.rstd[row];
-        float h[CH][N], g[CH][N];
+        float g[CH][N], h[CH][N], r[CH][N];
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+            const int c = (k * TPR + t) * N;
+            load_vals<float>(reinterpret_cast<const T *>(p.dY) + row * p.lddy + c, p.cols - c, g[k]);
+            load_vals<float>(reinterpret_cast<const T *>(p.H) + row * p.ldh + c, p.cols - c, h[k]);
+            if (p.dR) { load_vals<float>(reinterpret_cast<const T *>(p.dR) + row * p.lddr + c, p.cols - c, r[k]); }
+        }
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < CH; ++k)
         {
-            float dy[N];
-            s += grad_input<T>(p, row, (k * TPR + t) * N, dy, h[k], g[k]);
+            const int c = (k * TPR + t) * N;
+            float w[N];
+            load_weight<T>(p.weight, p.weight_f32, c, p.cols - c, w);
 #pragma unroll
-            for (int i = 0; i < N; ++i) { acc[k][i] += dy[i] * (h[k][i] * rstd); }
+            for (int i = 0; i < N; ++i)
+            {
+                acc[k][i] += g[k][i] * (h[k][i] * rstd);
+                g[k][i] *= w[i];
+                s += g[k][i] * h[k][i];                                      // 0 behind the row
+            }
         }
-        const float mean = row_sum<TPR>(s, sh, flip) / (float)p.cols;
-        const float coef = mean * rstd * rstd * rstd;
+        const float coef = row_sum<TPR>(s, sh, flip) / (float)p.cols * rstd * rstd * rstd;
 #pragma unroll
-        for (int k = 0; k < CH; ++k) { grad_output<T>(p, row, (k * TPR + t) * N, fk, rstd, coef, h[k], g[k]); }
+        for (int k = 0; k < CH; ++k)
+        {
+            const int c = (k * TPR + t) * N;
+#pragma unroll
+            for (int i = 0; i < N; ++i) { g[k][i] = g[k][i] * rstd - h[k][i] * coef + (p.dR ? r[k][i] : 0.0f); }
+            grad_store<T>(p, row, c, fk, g[k]);
+        }
     }
     if (!p.dW) { return; }
     float *out = p.work + (size_t)blockIdx.x * p.cols;
@@ -423,7 +488,13 @@ __global__ __launch_bounds__(NT) void norm_grad_wide_kernel(const NormGradParams
         {
             float dy[N], h[N], g[N];
             (void)grad_input<T>(p, row, c, dy, h, g);
-            grad_output<T>(p, row, c, fk, rstd, coef, h, g);
+            float r[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) { r[i] = 0.0f; }
+            if (p.dR) { load_vals<float>(reinterpret_cast<const T *>(p.dR) + row * p.lddr + c, p.cols - c, r); }
+#pragma unroll
+            for (int i = 0; i < N; ++i) { g[i] = g[i] * rstd - h[i] * coef + r[i]; }
+            grad_store<T>(p, row, c, fk, g);
         }
     }
 }
@@ -441,91 +512,135 @@ __global__ __launch_bounds__(NT) void norm_grad_weight_kernel(const NormGradPara
     p.work[(size_t)blockIdx.y * p.cols + c] = s;
 }
 
-// dW[c] = sum of the groups' partial sums: 32 columns a workgroup, 8 threads for each take every 8th group, their sums are added in
-// order
+// dW[c] = sum of the groups' partial sums: 32 columns a workgroup, 8 threads of 4 columns; 32 such rows of threads take every 32nd group,
+// and their sums are added in order.
 __global__ __launch_bounds__(NT) void norm_grad_reduce_kernel(const float *work, float *dW, int cols, int groups)
 {
-    __shared__ float sh[NT];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
-    float s = 0.0f;
-    if (c < cols) { for (int g = k; g < groups; g += 8) { s += work[(size_t)g * cols + c]; } }
-    sh[threadIdx.x] = s;
-    __syncthreads();
-    if (k == 0 && c < cols)
+    __shared__ float sh[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 7) * 4, k = threadIdx.x >> 3;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int g = k; g < groups; g += 32)
     {
-        for (int j = 1; j < 8; ++j) { s += sh[j * 32 + threadIdx.x]; }
-        dW[c] = s;
+        float v[4];
+        load_vals<float>(work + (size_t)g * cols + c, cols - c, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { s[i] += v[i]; }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { sh[k][(threadIdx.x & 7) * 4 + i] = s[i]; }
+    __syncthreads();
+    const int d = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && d < cols)
+    {
+        float t = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) { t += sh[j][threadIdx.x]; }
+        dW[d] = t;
     }
 }
 
 // ---- the quantizer ----
-// 16 lanes take a block of a row, 8 elements each.
-template <typename T>
-__global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, size_t rows, size_t cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, size_t nb)
+// 16 values of a block, already times its factor, to 16 bytes at q, or the first n of them
+__device__ __forceinline__ void store_e4m3_16(uint8_t *q, int n, const float (&x)[16], float f)
 {
-    const size_t units = rows * nb;
-    const int l = threadIdx.x & 15;
-    for (size_t u = (size_t)blockIdx.x * (NT / 16) + threadIdx.x / 16; u < units; u += (size_t)gridDim.x * (NT / 16))
-    {
-        const size_t row = u / nb, b = u - row * nb, c = b * ROWS_BLOCK + l * 8;
-        const int n = c < cols ? (int)min(cols - c, (size_t)8) : 0;
-        float x[8];
-        load_vals<float>(X + row * ldx + c, n, x);
-        unsigned amax = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { amax = max(amax, finite_bits(x[i])); }
-        const unsigned e = block_exponent(lanes_max<16>(amax));
-        store_e4m3(Q + row * ldq + c, n, x, block_factor(e));
-        if (l == 0) { S[row * lds + b] = (uint8_t)e; }
-    }
-}
-
-// The transpose's form: a workgroup reads 128 rows of 32 columns into LDS and writes 32 rows of one block; 8 threads take a column,
-// 16 of its values each.
-constexpr int QT_COLS = 32;
-template <typename T>
-__global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size_t ldx, size_t rows, size_t cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, unsigned ncb)
-{
-    __shared__ float sh[ROWS_BLOCK][QT_COLS + 1];
-    const unsigned rb = blockIdx.x / ncb;
-    const size_t r0 = (size_t)rb * ROWS_BLOCK, c0 = (size_t)(blockIdx.x - rb * ncb) * QT_COLS;
-    for (int i = threadIdx.x; i < ROWS_BLOCK * QT_COLS; i += NT)
-    {
-        const int r = i / QT_COLS, c = i % QT_COLS;
-        sh[r][c] = r0 + r < rows && c0 + c < cols ? (float)X[(r0 + r) * ldx + c0 + c] : 0.0f;
-    }
-    __syncthreads();
-    const int c = threadIdx.x / 8, g = threadIdx.x % 8;
-    float x[16];
-    unsigned amax = 0u;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) { x[i] = sh[g * 16 + i][c]; amax = max(amax, finite_bits(x[i])); }
-    const unsigned e = block_exponent(lanes_max<8>(amax));
-    if (c0 + c >= cols) { return; }
-    const float f = block_factor(e);
-    uint8_t *q = Q + (c0 + c) * ldq + r0 + g * 16;
-    const size_t left = rows > r0 + g * 16 ? rows - (r0 + g * 16) : 0;
     unsigned w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { w[i] = pack_e4m3(x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f); }
-    if (left >= 16) { *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]); }
+    if (n >= 16) { *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]); }
     else
     {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { if ((size_t)i < left) { q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4))); } }
+        for (int i = 0; i < 16; ++i) { if (i < n) { q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4))); } }
     }
-    if (g == 0) { S[(c0 + c) * lds + rb] = (uint8_t)e; }
+}
+
+// 8 lanes take a block of a row, 16 elements each; row and block move by fixed steps.
+template <typename T>
+__global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, size_t rows, int cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, int nb,
+                                                      size_t step_row, int step_b)
+{
+    constexpr int V = vec_of<T>();
+    const int l = threadIdx.x & 7;
+    const size_t first = (size_t)blockIdx.x * (NT / 8) + threadIdx.x / 8;
+    size_t row = first / (unsigned)nb;
+    int b = (int)(first - row * (unsigned)nb);
+    while (row < rows)
+    {
+        const int c = b * ROWS_BLOCK + l * 16;
+        float x[16];
+#pragma unroll
+        for (int k = 0; k < 16; k += V)
+        {
+            float v[V];
+            load_vals<float>(X + row * ldx + c + k, cols - c - k, v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { x[k + i] = v[i]; }
+        }
+        unsigned amax = 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { amax = max(amax, finite_bits(x[i])); }
+        const unsigned e = block_exponent(lanes_max<8>(amax));
+        store_e4m3_16(Q + row * ldq + c, cols - c, x, block_factor(e));
+        if (l == 0) { S[row * lds + b] = (uint8_t)e; }
+        row += step_row; b += step_b;
+        if (b >= nb) { b -= nb; ++row; }
+    }
+}
+
+// The transpose's form: a workgroup reads 128 rows of 64 columns into LDS and writes 64 rows of one block; 8 threads take a column,
+// 16 of its values each.  Rows of LDS are 65 words, so that neither the writing of rows nor the reading of columns piles up on banks.
+constexpr int QT_COLS = 64;
+template <typename T>
+__global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size_t ldx, size_t rows, size_t cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, unsigned ncb)
+{
+    constexpr int V = vec_of<T>(), VR = QT_COLS / V;                         // vectors of a row
+    __shared__ float sh[ROWS_BLOCK * (QT_COLS + 1)];
+    const unsigned rb = blockIdx.x / ncb;
+    const size_t r0 = (size_t)rb * ROWS_BLOCK, c0 = (size_t)(blockIdx.x - rb * ncb) * QT_COLS;
+    const int rleft = (int)min(rows - r0, (size_t)ROWS_BLOCK), cleft = (int)min(cols - c0, (size_t)QT_COLS);
+    float v[ROWS_BLOCK * VR / NT][V];
+#pragma unroll
+    for (int k = 0; k < ROWS_BLOCK * VR / NT; ++k)
+    {
+        const int i = k * NT + threadIdx.x, r = i / VR, c = (i % VR) * V;
+        load_vals<float>(X + (r0 + r) * ldx + c0 + c, r < rleft ? cleft - c : 0, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS_BLOCK * VR / NT; ++k)
+    {
+        const int i = k * NT + threadIdx.x, r = i / VR, c = (i % VR) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) { sh[r * (QT_COLS + 1) + c + j] = v[k][j]; }
+    }
+    __syncthreads();
+    const int g = threadIdx.x % 8;
+#pragma unroll
+    for (int k = 0; k < QT_COLS / (NT / 8); ++k)
+    {
+        const int c = k * (NT / 8) + threadIdx.x / 8;
+        float x[16];
+        unsigned amax = 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { x[i] = sh[(g * 16 + i) * (QT_COLS + 1) + c]; amax = max(amax, finite_bits(x[i])); }
+        const unsigned e = block_exponent(lanes_max<8>(amax));
+        if (c >= cleft) { continue; }
+        store_e4m3_16(Q + (c0 + c) * ldq + r0 + g * 16, rleft - g * 16, x, block_factor(e));
+        if (g == 0) { S[(c0 + c) * lds + rb] = (uint8_t)e; }
+    }
 }
 
 // ---- launches ----
-// Threads a row and vectors a thread from the width alone: a row that fits 16 or 64 lanes needs no barrier; up to 1024 threads x 4
+// Threads a row and vectors a thread: a row that fits 16 or 64 lanes needs no barrier, but where there are no more rows than CUs a wave
+// with several vectors a lane would be all that a CU has (1 x 2048 bf16: a wave 6.0 us, four waves 5.0); up to 1024 threads x 4
 // vectors hold a row (16 384 floats, 32 768 16-bit values), beyond that it is walked twice.
-#define ROWS_BY_WIDTH(T, cols, GO, WIDE)                                                                     \
+#define ROWS_BY_WIDTH(T, rows, cols, GO, WIDE)                                                               \
     do {                                                                                                     \
         const int nv_ = ((cols) + vec_of<T>() - 1) / vec_of<T>();                                            \
         if (nv_ <= 16) { GO(16, 1); }                                                                        \
         else if (sizeof(T) == 4 && nv_ <= 32) { GO(16, 2); }                                                 \
         else if (nv_ <= 64) { GO(64, 1); }                                                                   \
+        else if (nv_ <= 256 && (rows) <= 256) { GO(256, 1); }                                                \
         else if (nv_ <= 128) { GO(64, 2); }                                                                  \
         else if (nv_ <= 256) { GO(64, 4); }                                                                  \
         else if (nv_ <= 512) { GO(256, 2); }                                                                 \
@@ -534,7 +649,7 @@ __global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size
         else { WIDE; }                                                                                       \
     } while (0)
 
-constexpr size_t NORM_MAX_WG = 8192;
+constexpr size_t NORM_MAX_WG = 2048;                                       // 8 workgroups a CU: enough loads in flight, weights read seldom
 
 template <typename T>
 void norm_go(const NormParams &p, hipStream_t s)
@@ -545,7 +660,7 @@ void norm_go(const NormParams &p, hipStream_t s)
         const size_t g = (p.rows + rpw - 1) / rpw;                                                           \
         hipLaunchKernelGGL((norm_kernel<T, TPR, CH>), dim3((unsigned)(g < NORM_MAX_WG ? g : NORM_MAX_WG)), dim3(nth), 0, s, p); \
     } while (0)
-    ROWS_BY_WIDTH(T, p.cols, GO, hipLaunchKernelGGL(norm_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p));
+    ROWS_BY_WIDTH(T, p.rows, p.cols, GO, hipLaunchKernelGGL(norm_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p));
 #undef GO
 }
 
@@ -566,7 +681,7 @@ void norm_grad_go(const NormGradParams &p, hipStream_t s)
         if (p.dW && groups) { hipLaunchKernelGGL(norm_grad_weight_kernel<T>, dim3((unsigned)((p.cols + NT - 1) / NT), (unsigned)groups), dim3(NT), 0, s, p, groups); } \
         if (groups) { hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p); } \
     } while (0)
-    ROWS_BY_WIDTH(T, p.cols, GO, WIDE);
+    ROWS_BY_WIDTH(T, p.rows, p.cols, GO, WIDE);
 #undef WIDE
 #undef GO
     if (p.dW) { hipLaunchKernelGGL(norm_grad_reduce_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(NT), 0, s, p.work, p.dW, p.cols, groups); }
@@ -591,8 +706,8 @@ void quantize_go(size_t rows, size_t cols, const void *X, size_t ldx, uint8_t *Q
         hipLaunchKernelGGL(quantize_transpose_kernel<T>, dim3((unsigned)(nrb * ncb)), dim3(NT), 0, s, x, ldx, rows, cols, Q, ldq, S, lds, (unsigned)ncb);
         return;
     }
-    const size_t nb = (cols + ROWS_BLOCK - 1) / ROWS_BLOCK, want = (rows * nb + NT / 16 - 1) / (NT / 16);
-    hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)(want < 16384 ? want : 16384)), dim3(NT), 0, s, x, ldx, rows, cols, Q, ldq, S, lds, nb);
+    const size_t nb = (cols + ROWS_BLOCK - 1) / ROWS_BLOCK, want = (rows * nb + NT / 8 - 1) / (NT / 8), grid = want < 4096 ? want : 4096, width = grid * (NT / 8);
+    hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)grid), dim3(NT), 0, s, x, ldx, rows, (int)cols, Q, ldq, S, lds, (int)nb, width / nb, (int)(width % nb));
 }
 
 }  // namespace

@@ -37,6 +37,12 @@ __device__ __forceinline__ uint4 keep_bytes(uint4 v, int left)
     return v;
 }
 
+__device__ __forceinline__ v8i load_whole(const uint8_t *q)
+{
+    const int4 x = *reinterpret_cast<const int4 *>(q), y = *reinterpret_cast<const int4 *>(q + 64);
+    return v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+}
+
 // 32 bytes of a row from k on: 16 bytes at k and 16 at k + 64, zeros from K on
 __device__ __forceinline__ v8i load_frag(const uint8_t *row, size_t k, size_t K)
 {
@@ -57,8 +63,9 @@ __device__ __forceinline__ v8i load_frag(const uint8_t *row, size_t k, size_t K)
     return r;
 }
 
-// A workgroup computes 16 MT x 16 NN values; its WAVES waves split the k-steps and add their sums in wave order through LDS.
-// Operands come straight from memory.
+// Few values, any K: a workgroup computes 16 MT x 16 NN of them, its WAVES waves split the k-steps, and their sums are added in wave order
+// through LDS.  Operands come straight from memory: nothing is read twice that another workgroup's read would not have left in
+// L2.  With one row of A this is the reading of the weights.
 template <typename T, int MT, int NN, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void product_split_kernel(const ProductParams p, unsigned ntiles)
 {
@@ -66,12 +73,12 @@ __global__ __launch_bounds__(64 * WAVES) void product_split_kernel(const Product
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     const unsigned tm = blockIdx.x / ntiles, tn = blockIdx.x - tm * ntiles;
     const size_t m0 = (size_t)tm * 16 * MT, n0 = (size_t)tn * 16 * NN;
-    const int nb = (int)((p.K + ROWS_BLOCK - 1) / ROWS_BLOCK);
-    size_t ra[MT], rb[NN];
+    const int nb = (int)((p.K + ROWS_BLOCK - 1) / ROWS_BLOCK), whole = (int)(p.K / ROWS_BLOCK);
+    const uint8_t *A[MT], *B[NN], *SA[MT], *SB[NN];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) { const size_t r = m0 + 16 * i + l16; ra[i] = r < p.M ? r : p.M - 1; }
+    for (int i = 0; i < MT; ++i) { const size_t r = min(m0 + 16 * i + l16, p.M - 1); A[i] = p.A + r * p.lda + g * 16; SA[i] = p.SA + r * p.ldsa; }
 #pragma unroll
-    for (int i = 0; i < NN; ++i) { const size_t r = n0 + 16 * i + l16; rb[i] = r < p.N ? r : p.N - 1; }
+    for (int j = 0; j < NN; ++j) { const size_t r = min(n0 + 16 * j + l16, p.N - 1); B[j] = p.B + r * p.ldb + g * 16; SB[j] = p.SB + r * p.ldsb; }
     v4f acc[MT][NN];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -79,22 +86,26 @@ __global__ __launch_bounds__(64 * WAVES) void product_split_kernel(const Product
 #pragma unroll
         for (int j = 0; j < NN; ++j) { acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f}; }
     }
-    for (int b = wave; b < nb; b += WAVES)
+    auto step = [&](int b, bool cut)
     {
-        const size_t k = (size_t)b * ROWS_BLOCK + g * 16;
+        const size_t k = (size_t)b * ROWS_BLOCK;
         v8i fa[MT], fb[NN];
         int sa[MT], sb[NN];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) { fa[i] = load_frag(p.A + ra[i] * p.lda, k, p.K); sa[i] = p.SA[ra[i] * p.ldsa + b]; }
+        for (int j = 0; j < NN; ++j) { fb[j] = cut ? load_frag(B[j] - g * 16, k + g * 16, p.K) : load_whole(B[j] + k); sb[j] = SB[j][b]; }
 #pragma unroll
-        for (int i = 0; i < NN; ++i) { fb[i] = load_frag(p.B + rb[i] * p.ldb, k, p.K); sb[i] = p.SB[rb[i] * p.ldsb + b]; }
+        for (int i = 0; i < MT; ++i) { fa[i] = cut ? load_frag(A[i] - g * 16, k + g * 16, p.K) : load_whole(A[i] + k); sa[i] = SA[i][b]; }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
         {
 #pragma unroll
             for (int j = 0; j < NN; ++j) { acc[i][j] = mfma_scaled(fa[i], fb[j], acc[i][j], sa[i], sb[j]); }
         }
-    }
+    };
+    int b = wave;
+#pragma unroll 4
+    for (; b < whole; b += WAVES) { step(b, false); }
+    if (b < nb) { step(b, true); }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
     {
@@ -152,6 +163,11 @@ __device__ __forceinline__ void load_to_lds_at(const uint8_t *base, unsigned off
 {
     asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base), "n"(STEP) : "memory", "m0", "scc");
 }
+// a dword a lane from base + off into LDS at lds + 4 lane
+__device__ __forceinline__ void load_dword_to_lds(const uint8_t *base, unsigned off, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
 // a dword a lane from each of two arrays into LDS at lds + 4 lane and 1024 behind, or nothing, without a branch: the loads of no lane
 __device__ __forceinline__ void load_dwords_to_lds_if(bool yes, const uint8_t *one, unsigned off1, const uint8_t *two, unsigned off2, unsigned lds)
 {
@@ -162,78 +178,65 @@ __device__ __forceinline__ void load_dwords_to_lds_if(bool yes, const uint8_t *o
                  : "=&s"(all) : "s"(lanes), "s"(lds), "v"(off1), "s"(one), "v"(off2), "s"(two) : "memory", "m0", "scc");
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
+//
+// STAGES stages are in LDS: one is read while the others arrive.  Scales go through LDS too, a dword of four k-steps for each row.
+template <typename T, int TM, int TN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
 {
-    constexpr int NTH = 64 * WM * WN, MT = TM / WM / 16, NN = TN / WN / 16, STAGE = (TM + TN) * 128;
-    constexpr int LA = TM * 8 / NTH, LB = TN * 8 / NTH;                      // 16-byte loads a thread makes for a stage
+    constexpr int NTH = 64 * WM * WN, MT = TM / WM / 16, NN = TN / WN / 16, ROWS = TM + TN, STAGE = ROWS * 128;
+    constexpr int LA = TM * 8 / NTH, LB = TN * 8 / NTH, LOADS = LA + LB;     // 16-byte loads a thread makes for a stage
+    constexpr int LS = (ROWS + NTH - 1) / NTH;                               // and dwords for four stages' scales
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g = lane >> 4;
-    const int wm = wave / WN, wn = wave % WN;
+    uint8_t *lds_scales = lds + STAGES * STAGE;
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
 
-    // XCDs take workgroups in turn: each gets a run of consecutive tiles, which walk 8 tiles of rows at a time so that the 32 tiles an XCD
+    // XCDs take workgroups in turn: each gets a run of consecutive tiles, which walk 8 tiles of rows at a time so that the tiles an XCD
     // works on share their rows of A and B in its L2
     const unsigned total = tiles_m * tiles_n, per = (total + 7) / 8;
     const unsigned tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (tile >= total) { return; }
+    if ((blockIdx.x >> 3) >= per || tile >= total) { return; }
     const unsigned band = tile / (8 * tiles_n), in = tile - band * 8 * tiles_n, bh = min(8u, tiles_m - band * 8);
     const size_t m0 = (size_t)(band * 8 + in % bh) * TM, n0 = (size_t)(in / bh) * TN;
 
     const int nb = (int)((p.K + 127) / 128);
     const int am = (int)min(p.M - m0, (size_t)TM) - 1, bm = (int)min(p.N - n0, (size_t)TN) - 1;     // last row of the tile that exists
-    const uint8_t *A = p.A + m0 * p.lda, *B = p.B + n0 * p.ldb;
-    const unsigned lda = (unsigned)p.lda, ldb = (unsigned)p.ldb;
-    unsigned oa[LA], ob[LB];
+    const uint8_t *A = p.A + m0 * p.lda, *B = p.B + n0 * p.ldb, *SA = p.SA + m0 * p.ldsa, *SB = p.SB + n0 * p.ldsb;
+    const int lr = tid >> 3, ca = (tid & 7) ^ swizzle_a(lr), cb = (tid & 7) ^ swizzle_b(lr);         // NTH / 8 rows a load, a multiple of 16
+    unsigned oa[LA], ob[LB], os[LS];
 #pragma unroll
-    for (int i = 0; i < LA; ++i)
-    {
-        const int row = i * (NTH / 8) + tid / 8;
-        oa[i] = (unsigned)min(row, am) * lda + (unsigned)(((tid & 7) ^ swizzle_a(row)) * 16);
-    }
+    for (int i = 0; i < LA; ++i) { oa[i] = (unsigned)min(i * (NTH / 8) + lr, am) * (unsigned)p.lda + (unsigned)(ca * 16); }
 #pragma unroll
-    for (int i = 0; i < LB; ++i)
+    for (int i = 0; i < LB; ++i) { ob[i] = (unsigned)min(i * (NTH / 8) + lr, bm) * (unsigned)p.ldb + (unsigned)(cb * 16); }
+#pragma unroll
+    for (int i = 0; i < LS; ++i)
     {
-        const int row = i * (NTH / 8) + tid / 8;
-        ob[i] = (unsigned)min(row, bm) * ldb + (unsigned)(((tid & 7) ^ swizzle_b(row)) * 16);
+        const int r = i * NTH + tid;                                         // a wave's 64 rows are A's or B's: TM is a multiple of 64
+        os[i] = r < TM ? (unsigned)min(r, am) * (unsigned)p.ldsa : (unsigned)min(r - TM, bm) * (unsigned)p.ldsb;
     }
-    const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds + (unsigned)wave * 1024u);
+    const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds);
     const int last = (int)(p.K - (size_t)(nb - 1) * 128);                    // bytes of the last k-step: 1 ... 128
 
     // chunks that start at or behind K are fetched from the row's first bytes (they are cleared in LDS below)
-    auto fetch = [&](int kb, int stage)
+    auto fetch = [&](int kb)
     {
         const bool cut = kb == nb - 1 && last < 128;
-        const size_t k = (size_t)kb * 128;
-        const unsigned dst = lds0 + (unsigned)(stage * STAGE);
+        const unsigned da = cut && ca * 16 >= last ? (unsigned)(ca * 16) : 0u, db = cut && cb * 16 >= last ? (unsigned)(cb * 16) : 0u;
+        const uint8_t *a = A + (size_t)kb * 128, *b = B + (size_t)kb * 128;
+        const unsigned dst = base + (unsigned)((kb % STAGES) * STAGE + wave * 1024);
 #pragma unroll
-        for (int i = 0; i < LA; ++i)
-        {
-            const int row = i * (NTH / 8) + tid / 8, c = (tid & 7) ^ swizzle_a(row);
-            const unsigned o = cut && c * 16 >= last ? oa[i] - (unsigned)(c * 16) : oa[i];
-            load_to_lds(A + k, o, dst + (unsigned)(i * (NTH * 16)));
-        }
+        for (int i = 0; i < LA; ++i) { load_to_lds(a, oa[i] - da, dst + (unsigned)(i * (NTH * 16))); }
 #pragma unroll
-        for (int i = 0; i < LB; ++i)
-        {
-            const int row = i * (NTH / 8) + tid / 8, c = (tid & 7) ^ swizzle_b(row);
-            const unsigned o = cut && c * 16 >= last ? ob[i] - (unsigned)(c * 16) : ob[i];
-            load_to_lds(B + k, o, dst + (unsigned)(TM * 128 + i * (NTH * 16)));
-        }
+        for (int i = 0; i < LB; ++i) { load_to_lds(b, ob[i] - db, dst + (unsigned)(TM * 128 + i * (NTH * 16))); }
     };
-
-    // scales: a dword holds a row's next four k-steps
-    const uint8_t *SA[MT], *SB[NN];
-    unsigned sa[MT], sb[NN], na[MT], nbx[NN];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) { SA[i] = p.SA + (m0 + (size_t)min(wm * (TM / WM) + 16 * i + l16, am)) * p.ldsa; }
-#pragma unroll
-    for (int j = 0; j < NN; ++j) { SB[j] = p.SB + (n0 + (size_t)min(wn * (TN / WN) + 32 * (j >> 1) + 4 * (j & 1) + 8 * (l16 >> 2) + (l16 & 3), bm)) * p.ldsb; }
-    auto fetch_scales = [&](int kb)
+    auto fetch_scales = [&](int kb)                                          // before a group of four's first stage
     {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) { na[i] = *reinterpret_cast<const unsigned *>(SA[i] + kb); }
-#pragma unroll
-        for (int j = 0; j < NN; ++j) { nbx[j] = *reinterpret_cast<const unsigned *>(SB[j] + kb); }
+        for (int i = 0; i < LS; ++i)
+        {
+            const int r0 = i * NTH + wave * 64;
+            if (r0 < ROWS) { load_dword_to_lds((r0 < TM ? SA : SB) + kb, os[i], base + (unsigned)(STAGES * STAGE + (kb >> 2 & 1) * (ROWS * 4) + r0 * 4)); }
+        }
     };
 
     v4f acc[MT][NN];
@@ -243,23 +246,26 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
 #pragma unroll
         for (int j = 0; j < NN; ++j) { acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f}; }
     }
+    // row 16 i + l16 of A: chunk g ^ (l16 & 7); row 32 (j / 2) + 4 (j % 2) + 8 (l16 / 4) + l16 % 4 of B: the same
+    const int place = (g ^ (l16 & 7)) * 16, arow = wm * (TM / WM) + l16, brow = wn * (TN / WN) + 8 * (l16 >> 2) + (l16 & 3);
+    const int qa = arow * 128 + place, qb = (TM + brow) * 128 + place;
 
-    if (nb > 0) { fetch_scales(0); fetch(0, 0); }
+    for (int kb = 0; kb < STAGES - 1 && kb < nb; ++kb)
+    {
+        if ((kb & 3) == 0) { fetch_scales(kb); }
+        fetch(kb);
+    }
     for (int kb = 0; kb < nb; ++kb)
     {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // a barrier alone does not wait for this wave's loads into LDS
-        __syncthreads();                                                     // this stage is in LDS, the other one is free
-        if ((kb & 3) == 0)
-        {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) { sa[i] = na[i]; }
-#pragma unroll
-            for (int j = 0; j < NN; ++j) { sb[j] = nbx[j]; }
-        }
-        uint8_t *st = lds + (kb & 1) * STAGE;
+        // this wave's loads of the stage have arrived: the STAGES - 2 stages behind it may be on their way, near the end everything is
+        // waited for; a barrier alone does not wait for loads into LDS
+        if (kb + STAGES - 1 <= nb) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * LOADS) : "memory"); }
+        else { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+        __syncthreads();                                                     // the stage is in LDS, the one before it is free
+        uint8_t *st = lds + (kb % STAGES) * STAGE;
         if (kb == nb - 1 && last < 128)
         {
-            for (int r = tid; r < TM + TN; r += NTH)
+            for (int r = tid; r < ROWS; r += NTH)
             {
                 const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
                 for (int c = last / 16; c < 8; ++c)
@@ -270,36 +276,32 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
             }
             __syncthreads();
         }
-        if (kb + 1 < nb)
+        const int ahead = kb + STAGES - 1;
+        if (ahead < nb)
         {
-            if ((kb & 3) == 3) { fetch_scales(kb + 1); }
-            fetch(kb + 1, (kb + 1) & 1);
+            if ((ahead & 3) == 0) { fetch_scales(ahead); }
+            fetch(ahead);
         }
+        const uint8_t *sc = lds_scales + (kb >> 2 & 1) * (ROWS * 4) + (kb & 3);
         v8i fb[NN];
+        int sb[NN];
 #pragma unroll
         for (int j = 0; j < NN; ++j)
         {
-            const int row = wn * (TN / WN) + 32 * (j >> 1) + 4 * (j & 1) + 8 * (l16 >> 2) + (l16 & 3);
-            const uint8_t *q = st + TM * 128 + row * 128;
-            const int c = g ^ swizzle_b(row);
-            const int4 x = *reinterpret_cast<const int4 *>(q + c * 16), y = *reinterpret_cast<const int4 *>(q + (c ^ 4) * 16);
+            const int o = (j >> 1) * 4096 + (j & 1) * 512;
+            const int4 x = *reinterpret_cast<const int4 *>(st + qb + o), y = *reinterpret_cast<const int4 *>(st + (qb ^ 64) + o);
             fb[j] = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            sb[j] = sc[(TM + brow) * 4 + (j >> 1) * 128 + (j & 1) * 16];
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
         {
-            const int row = wm * (TM / WM) + 16 * i + l16;
-            const uint8_t *q = st + row * 128;
-            const int c = g ^ swizzle_a(row);
-            const int4 x = *reinterpret_cast<const int4 *>(q + c * 16), y = *reinterpret_cast<const int4 *>(q + (c ^ 4) * 16);
+            const int4 x = *reinterpret_cast<const int4 *>(st + qa + i * 2048), y = *reinterpret_cast<const int4 *>(st + (qa ^ 64) + i * 2048);
             const v8i fa = v8i{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            const int sa = sc[arow * 4 + i * 64];
 #pragma unroll
-            for (int j = 0; j < NN; ++j) { acc[i][j] = mfma_scaled(fb[j], fa, acc[i][j], (int)sb[j], (int)sa[i]); }
+            for (int j = 0; j < NN; ++j) { acc[i][j] = mfma_scaled(fb[j], fa, acc[i][j], sb[j], sa); }
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) { sa[i] >>= 8; }
-#pragma unroll
-        for (int j = 0; j < NN; ++j) { sb[j] >>= 8; }
     }
 
     const size_t n = n0 + (size_t)(wn * (TN / WN) + 8 * g);
@@ -562,28 +564,47 @@ hipError_t stream_go(const ProductParams &p, hipStream_t s)
     return hipSuccess;
 }
 
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, int TM, int TN, int WM, int WN, int STAGES>
 hipError_t tile_go(const ProductParams &p, hipStream_t s)
 {
-    constexpr int LDS = 2 * (TM + TN) * 128;
-    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<T, TM, TN, WM, WN>);
+    constexpr int LDS = STAGES * (TM + TN) * 128 + 2 * (TM + TN) * 4;
+    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<T, TM, TN, WM, WN, STAGES>);
     const hipError_t e = opt_in_lds_once(k, LDS);
     if (e != hipSuccess) { return e; }
     const unsigned tm = (unsigned)((p.M + TM - 1) / TM), tn = (unsigned)((p.N + TN - 1) / TN);
-    hipLaunchKernelGGL((product_tile_kernel<T, TM, TN, WM, WN>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN), LDS, s, p, tm, tn);
+    hipLaunchKernelGGL((product_tile_kernel<T, TM, TN, WM, WN, STAGES>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN), LDS, s, p, tm, tn);
     return hipSuccess;
 }
 
+template <typename T, int MT, int NN, int WAVES>
+hipError_t split_go(const ProductParams &p, hipStream_t s)
+{
+    const size_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 16 * NN - 1) / (16 * NN);
+    hipLaunchKernelGGL((product_split_kernel<T, MT, NN, WAVES>), dim3((unsigned)(tm * tn)), dim3(64 * WAVES), 0, s, p, (unsigned)tn);
+    return hipSuccess;
+}
+
+size_t tiles(const ProductParams &p, size_t tm, size_t tn) { return ((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn); }
+
+// Which kernel: the largest tile that still gives the 256 CUs about one each, since a value then costs the fewest operand bytes.
+// Measured, us (rows x columns x k): the chosen kernel / the next larger tile / the next smaller one
+//   stream 256 x 256   4096 x 4096 x 1024 (256 tiles)    24.3 / - / 26.0       2048 fewer columns (128 tiles, k 4096): 46.4, 128 x 128: 34.8
+//   128 x 128          7984 x 1024 x 2048 (504)          20.6 / 28.7 / 25.4    2048 x 2048 x 2048 (256): 15.9, 128 x 64: 14.0
+//   128 x 64           2048 x 1024 x 7984 (256)          35.4 / 55.0 / 42.7    1024 x 1024 x 1024 (128): 6.9, 64 x 64: 5.6
+//   64 x 64            1024 x 1024 x 1024 (256)          5.6 / 6.9 / 11.3      512 x 512 x 512 (64): 4.4, split 32 x 32: 3.9
+//   split 32 x 32      64 x 2048 x 2048 (128)            6.8 / 7.8 / 6.6
+//   split 16 x 16      1 x 8192 x 8192                   15.2 (4.4 TB/s of weights) / 19.2
 template <typename T>
 hipError_t product_go(const ProductParams &p, hipStream_t s)
 {
+    if (p.M <= 16) { return p.K <= 1024 ? split_go<T, 1, 1, 8>(p, s) : split_go<T, 1, 1, 16>(p, s); }      // 16 k-steps give 16 waves one each
     // rows of a tile are addressed in 32 bits from its first
-    const bool near = p.lda < ((size_t)1 << 23) && p.ldb < ((size_t)1 << 23) && p.ldsa < ((size_t)1 << 23) && p.ldsb < ((size_t)1 << 23);
-    if (near && p.M >= 256 && p.N >= 256 && p.K > 384 && ((p.M + 255) / 256) * ((p.N + 255) / 256) >= 128) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
-    if (near && ((p.M + 127) / 128) * ((p.N + 127) / 128) >= 64) { return tile_go<T, 128, 128, 2, 2>(p, s); }
-    const size_t tm = (p.M + 31) / 32, tn = (p.N + 31) / 32;
-    hipLaunchKernelGGL((product_split_kernel<T, 2, 2, 4>), dim3((unsigned)(tm * tn)), dim3(256), 0, s, p, (unsigned)tn);
-    return hipSuccess;
+    const bool near = p.K > 0 && p.lda < ((size_t)1 << 23) && p.ldb < ((size_t)1 << 23) && p.ldsa < ((size_t)1 << 23) && p.ldsb < ((size_t)1 << 23);
+    if (near && p.M >= 256 && p.N >= 256 && p.K > 384 && tiles(p, 256, 256) >= 240) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
+    if (near && tiles(p, 128, 128) >= 384) { return tile_go<T, 128, 128, 2, 2, 2>(p, s); }
+    if (near && tiles(p, 128, 64) >= 192) { return tile_go<T, 128, 64, 2, 2, 3>(p, s); }
+    if (near && tiles(p, 64, 64) >= 160) { return tile_go<T, 64, 64, 2, 2, 3>(p, s); }
+    return split_go<T, 2, 2, 8>(p, s);
 }
 
 }  // namespace
