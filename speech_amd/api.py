@@ -423,62 +423,78 @@ class Batch:
 # stream), write into the tensors they are given and allocate nothing.  A tensor that torch may reuse before the stream gets to
 # the call has to be kept, or recorded on that stream, by the caller.
 
-_ROWS_TYPES = {"torch.float32": _lib.F32, "torch.bfloat16": _lib.BF16, "torch.float16": _lib.F16, "torch.float64": _lib.F64}
-_HELD = ("torch.uint8", "torch.float8_e4m3fn")
-_SCALES = ("torch.uint8", "torch.float8_e8m0fnu")
+_ROWS = None
 
 
-def _rows_type(t, what, f64=False):
-    code = _ROWS_TYPES.get(str(t.dtype))
+class _RowsTypes:
+    """what the checks below compare with, made once torch is there: a call is to cost microseconds"""
+
+    def __init__(self):
+        import torch
+        self.lib = _lib.load()
+        self.f32 = torch.float32
+        self.codes = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float64: _lib.F64}
+        self.held = (torch.float8_e4m3fn, torch.uint8)
+        self.scales = (torch.uint8, torch.float8_e8m0fnu)
+        self.bytes = (torch.uint8,)
+        self.numbers = (torch.int64, torch.uint64)
+
+
+def _rows(t, what, f64=False):
+    """(types, dtype code, dtype, device) of a call's leading matrix"""
+    global _ROWS
+    if _ROWS is None:
+        _ROWS = _RowsTypes()
+    dtype = t.dtype
+    code = _ROWS.codes.get(dtype)
     if code is None or (code == _lib.F64 and not f64):
-        raise ValueError("%s must have dtype float32, bfloat16%s, got %s" % (what, ", float16 or float64" if f64 else " or float16", t.dtype))
-    return code
+        raise ValueError("%s must have dtype float32, bfloat16%s, got %s" % (what, ", float16 or float64" if f64 else " or float16", dtype))
+    if t.dim() != 2:
+        raise ValueError("%s must be a matrix, got shape %s" % (what, tuple(t.shape)))
+    return _ROWS, code, (dtype,), t.get_device()
+
+
+def _on(t, what, device, dtypes):
+    if device < 0 or t.get_device() != device:
+        raise ValueError("%s must be on cuda:%d, got %s" % (what, max(device, 0), t.device))
+    if t.dtype not in dtypes:
+        raise ValueError("%s must have dtype %s, got %s" % (what, " or ".join(str(d)[6:] for d in dtypes), t.dtype))
 
 
 def _rows_arg(t, what, device, dtypes, rows, cols, pad=1):
     """(pointer, row stride) of a rows x cols matrix after checking what the C ABI cannot: device, dtype, shape, strides, and that the
     memory behind the last row reaches up to a multiple of `pad` columns"""
-    if not t.is_cuda or t.get_device() != device:
-        raise ValueError("%s must be on cuda:%d, got %s" % (what, device, t.device))
-    if str(t.dtype) not in dtypes:
-        raise ValueError("%s must have dtype %s, got %s" % (what, " or ".join(d[6:] for d in dtypes), t.dtype))
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.get_device() != device or t.dtype not in dtypes or device < 0:
+        _on(t, what, device, dtypes)
+    if t.shape != (rows, cols):
         raise ValueError("%s must have shape (%d, %d), got %s" % (what, rows, cols, tuple(t.shape)))
     ld, unit = t.stride()
-    if cols > 1 and unit != 1:
+    if unit != 1 and cols > 1:
         raise ValueError("%s must have unit column stride, got %d" % (what, unit))
-    full = -(-cols // pad) * pad
+    full = cols if pad == 1 else -(-cols // pad) * pad
     if rows <= 1 or cols == 0:
         ld = full
     elif ld < cols or (pad > 1 and ld % pad):
         raise ValueError("%s has a row stride of %d for %d columns%s" % (what, ld, cols, "" if pad == 1 else ": a multiple of %d is needed" % pad))
-    if pad > 1 and rows and cols:
-        if t.storage_offset() + (rows - 1) * ld + full > t.untyped_storage().nbytes() or t.data_ptr() % pad:
-            raise ValueError("%s needs rows that start on %d bytes and have memory up to the next %d (see held)" % (what, pad, pad))
-    return t.data_ptr(), ld
+    p = t.data_ptr()
+    if pad > 1 and rows and cols and (t.storage_offset() + (rows - 1) * ld + full > t.untyped_storage().nbytes() or p % pad):
+        raise ValueError("%s needs rows that start on %d bytes and have memory up to the next %d (see held)" % (what, pad, pad))
+    return p, ld
 
 
 def _vector_arg(t, what, device, dtypes, n):
-    if not t.is_cuda or t.get_device() != device:
-        raise ValueError("%s must be on cuda:%d, got %s" % (what, device, t.device))
-    if str(t.dtype) not in dtypes:
-        raise ValueError("%s must have dtype %s, got %s" % (what, " or ".join(d[6:] for d in dtypes), t.dtype))
-    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    _on(t, what, device, dtypes)
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         raise ValueError("%s must be a contiguous vector of %d elements, got %s" % (what, n, tuple(t.shape)))
     return t.data_ptr()
 
 
-def _drop_arg(p, seed, step, keys, device, rows):
-    """speech_drop, or None where nothing is dropped"""
-    p = float(p)
+def _drop_arg(types, p, seed, step, keys, device, rows):
+    """speech_drop; with p = 0 nothing else matters"""
     if p == 0.0:
-        return None
-    d = _lib.SpeechDrop(p, int(seed) & 0xFFFFFFFFFFFFFFFF, None, None)
-    if step is not None:
-        d.step = _vector_arg(step.reshape(-1), "step", device, ("torch.int64", "torch.uint64"), 1)
-    if keys is not None:
-        d.keys = _vector_arg(keys, "keys", device, ("torch.int64", "torch.uint64"), rows)
-    return d
+        return _lib.SpeechDrop()
+    return _lib.SpeechDrop(p, int(seed) & 0xFFFFFFFFFFFFFFFF, None if step is None else _vector_arg(step.reshape(-1), "step", device, types.numbers, 1),
+                           None if keys is None else _vector_arg(keys, "keys", device, types.numbers, rows))
 
 
 def _rows_check(rc):
@@ -498,29 +514,30 @@ def held(rows, cols, device="cuda"):
 def dropout(X, Y, p, seed, step=None, keys=None, stream=None):
     """Y = X / (1 - p) where 32 random bits keyed by (seed + step, keys[row], column) say so, else 0; Y may be X.  The same call
     on a gradient is the backward pass.  step: an int64 tensor of one element on the device, added to the seed when the kernel runs"""
-    code = _rows_type(X, "X", f64=True)
+    types, code, same, dev = _rows(X, "X", f64=True)
     rows, cols = X.shape
-    dev = X.get_device()
-    xp, ldx = _rows_arg(X, "X", dev, (str(X.dtype),), rows, cols)
-    yp, ldy = _rows_arg(Y, "Y", dev, (str(X.dtype),), rows, cols)
-    d = _drop_arg(p, seed, step, keys, dev, rows) or _lib.SpeechDrop(0.0, 0, None, None)
-    _rows_check(_lib.load().speech_rows_dropout(dev, code, rows, cols, xp, ldx, yp, ldy, C.byref(d), stream or None))
+    xp, ldx = _rows_arg(X, "X", dev, same, rows, cols)
+    yp, ldy = _rows_arg(Y, "Y", dev, same, rows, cols)
+    d = _drop_arg(types, p, seed, step, keys, dev, rows)
+    _rows_check(types.lib.speech_rows_dropout(dev, code, rows, cols, xp, ldx, yp, ldy, C.byref(d), stream))
+
+
+def _weight_arg(types, weight, same, dev, cols):
+    return _vector_arg(weight, "weight", dev, same + (types.f32,), cols), int(weight.dtype is types.f32)
 
 
 def rms_norm(X, weight=None, eps=1e-6, residual=None, H=None, Y=None, Q=None, S=None, rstd=None, p=0.0, seed=0, step=None, keys=None, stream=None):
     """h = residual + dropout(X) -> H; h / sqrt(mean(h^2) + eps) * weight -> Y, or in 8-bit form -> (Q, S); 1 / sqrt(...) -> rstd.
     weight: X's dtype or float32.  H may be X or residual (in place)"""
-    code = _rows_type(X, "X")
+    types, code, same, dev = _rows(X, "X")
     rows, cols = X.shape
-    dev = X.get_device()
-    same = (str(X.dtype),)
-    a = _lib.SpeechNorm(dtype=code, rows=rows, cols=cols, eps=float(eps))
+    a = _lib.SpeechNorm()
+    a.dtype, a.rows, a.cols, a.eps = code, rows, cols, eps
     a.X, a.ldx = _rows_arg(X, "X", dev, same, rows, cols)
     if residual is not None:
         a.R, a.ldr = _rows_arg(residual, "residual", dev, same, rows, cols)
     if weight is not None:
-        a.weight = _vector_arg(weight, "weight", dev, same + ("torch.float32",), cols)
-        a.weight_f32 = int(str(weight.dtype) == "torch.float32")
+        a.weight, a.weight_f32 = _weight_arg(types, weight, same, dev, cols)
     if H is not None:
         a.H, a.ldh = _rows_arg(H, "H", dev, same, rows, cols)
     if Y is not None:
@@ -528,14 +545,13 @@ def rms_norm(X, weight=None, eps=1e-6, residual=None, H=None, Y=None, Q=None, S=
     if Q is not None:
         if S is None:
             raise ValueError("Q needs S")
-        a.Q, a.ldq = _rows_arg(Q, "Q", dev, _HELD, rows, cols, 16)
-        a.S, a.lds = _rows_arg(S, "S", dev, _SCALES, rows, -(-cols // 128), 4)
+        a.Q, a.ldq = _rows_arg(Q, "Q", dev, types.held, rows, cols, 16)
+        a.S, a.lds = _rows_arg(S, "S", dev, types.scales, rows, -(-cols // 128), 4)
     if rstd is not None:
-        a.rstd = _vector_arg(rstd, "rstd", dev, ("torch.float32",), rows)
-    d = _drop_arg(p, seed, step, keys, dev, rows)
-    if d is not None:
-        a.drop = C.pointer(d)
-    _rows_check(_lib.load().speech_rows_rms_norm(dev, C.byref(a), stream or None))
+        a.rstd = _vector_arg(rstd, "rstd", dev, (types.f32,), rows)
+    if p != 0.0:
+        a.drop = C.pointer(_drop_arg(types, p, seed, step, keys, dev, rows))
+    _rows_check(types.lib.speech_rows_rms_norm(dev, C.byref(a), stream))
 
 
 def rms_norm_work(rows, cols):
@@ -549,17 +565,15 @@ def rms_norm_backward(dY, H, weight, rstd, dH=None, dR=None, dX=None, dW=None, w
     """gradients of rms_norm from dY, the H and rstd it left, and dR, what reaches H on the residual stream's own way: dH (of the
     residual stream; of X where nothing was dropped), dX (of the dropped X), dW (float32).  work: a uint8 tensor of
     rms_norm_work(rows, cols) bytes at least, not used by another call in flight"""
-    code = _rows_type(H, "H")
+    types, code, same, dev = _rows(H, "H")
     rows, cols = H.shape
-    dev = H.get_device()
-    same = (str(H.dtype),)
-    a = _lib.SpeechNormGrad(dtype=code, rows=rows, cols=cols)
+    a = _lib.SpeechNormGrad()
+    a.dtype, a.rows, a.cols = code, rows, cols
     a.dY, a.lddy = _rows_arg(dY, "dY", dev, same, rows, cols)
     a.H, a.ldh = _rows_arg(H, "H", dev, same, rows, cols)
-    a.rstd = _vector_arg(rstd, "rstd", dev, ("torch.float32",), rows)
+    a.rstd = _vector_arg(rstd, "rstd", dev, (types.f32,), rows)
     if weight is not None:
-        a.weight = _vector_arg(weight, "weight", dev, same + ("torch.float32",), cols)
-        a.weight_f32 = int(str(weight.dtype) == "torch.float32")
+        a.weight, a.weight_f32 = _weight_arg(types, weight, same, dev, cols)
     if dR is not None:
         a.dR, a.lddr = _rows_arg(dR, "dR", dev, same, rows, cols)
     if dH is not None:
@@ -567,42 +581,39 @@ def rms_norm_backward(dY, H, weight, rstd, dH=None, dR=None, dX=None, dW=None, w
     if dX is not None:
         a.dX, a.lddx = _rows_arg(dX, "dX", dev, same, rows, cols)
     if dW is not None:
-        a.dW = _vector_arg(dW, "dW", dev, ("torch.float32",), cols)
+        a.dW = _vector_arg(dW, "dW", dev, (types.f32,), cols)
         if work is not None:
-            a.work, a.work_bytes = _vector_arg(work, "work", dev, ("torch.uint8",), work.numel()), work.numel()
-    d = _drop_arg(p, seed, step, keys, dev, rows)
-    if d is not None:
-        a.drop = C.pointer(d)
-    _rows_check(_lib.load().speech_rows_rms_norm_backward(dev, C.byref(a), stream or None))
+            a.work, a.work_bytes = _vector_arg(work, "work", dev, types.bytes, work.numel()), work.numel()
+    if p != 0.0:
+        a.drop = C.pointer(_drop_arg(types, p, seed, step, keys, dev, rows))
+    _rows_check(types.lib.speech_rows_rms_norm_backward(dev, C.byref(a), stream))
 
 
 def quantize(X, Q, S, transpose=False, stream=None):
     """(Q, S) = X in 8-bit form (see held): e4m3 values and a power-of-two scale for each 128 columns; transpose: X's transpose"""
-    code = _rows_type(X, "X")
+    types, code, same, dev = _rows(X, "X")
     rows, cols = X.shape
-    dev = X.get_device()
-    xp, ldx = _rows_arg(X, "X", dev, (str(X.dtype),), rows, cols)
+    xp, ldx = _rows_arg(X, "X", dev, same, rows, cols)
     r, c = (cols, rows) if transpose else (rows, cols)
-    qp, ldq = _rows_arg(Q, "Q", dev, _HELD, r, c, 16)
-    sp, lds = _rows_arg(S, "S", dev, _SCALES, r, -(-c // 128), 4)
-    _rows_check(_lib.load().speech_rows_quantize(dev, code, rows, cols, xp, ldx, qp, ldq, sp, lds, int(bool(transpose)), stream or None))
+    qp, ldq = _rows_arg(Q, "Q", dev, types.held, r, c, 16)
+    sp, lds = _rows_arg(S, "S", dev, types.scales, r, -(-c // 128), 4)
+    _rows_check(types.lib.speech_rows_quantize(dev, code, rows, cols, xp, ldx, qp, ldq, sp, lds, 1 if transpose else 0, stream))
 
 
 def product(A, SA, B, SB, Y, bias=None, stream=None):
     """Y = A B^T + bias for A (rows x k) and B (columns x k, a weight matrix with a row for each output) in 8-bit form; Y bfloat16 or
     float16, bias float32"""
-    code = _rows_type(Y, "Y")                                  # float32 is refused by the C side
+    types, code, same, dev = _rows(Y, "Y")                     # float32 is refused by the C side
     rows, cols = Y.shape
     k = A.shape[1]
-    dev = Y.get_device()
     nb = -(-k // 128)
-    ap, lda = _rows_arg(A, "A", dev, _HELD, rows, k, 16)
-    sa, ldsa = _rows_arg(SA, "SA", dev, _SCALES, rows, nb, 4)
-    bp, ldb = _rows_arg(B, "B", dev, _HELD, cols, k, 16)
-    sb, ldsb = _rows_arg(SB, "SB", dev, _SCALES, cols, nb, 4)
-    yp, ldy = _rows_arg(Y, "Y", dev, (str(Y.dtype),), rows, cols)
-    bias_p = _vector_arg(bias, "bias", dev, ("torch.float32",), cols) if bias is not None else None
-    _rows_check(_lib.load().speech_rows_product(dev, code, rows, cols, k, ap, lda, sa, ldsa, bp, ldb, sb, ldsb, bias_p, yp, ldy, stream or None))
+    ap, lda = _rows_arg(A, "A", dev, types.held, rows, k, 16)
+    sa, ldsa = _rows_arg(SA, "SA", dev, types.scales, rows, nb, 4)
+    bp, ldb = _rows_arg(B, "B", dev, types.held, cols, k, 16)
+    sb, ldsb = _rows_arg(SB, "SB", dev, types.scales, cols, nb, 4)
+    yp, ldy = _rows_arg(Y, "Y", dev, same, rows, cols)
+    _rows_check(types.lib.speech_rows_product(dev, code, rows, cols, k, ap, lda, sa, ldsa, bp, ldb, sb, ldsb,
+                                              None if bias is None else _vector_arg(bias, "bias", dev, (types.f32,), cols), yp, ldy, stream))
 
 
 def merge_stats(s, q, n, group=None):

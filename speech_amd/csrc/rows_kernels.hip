@@ -383,8 +383,9 @@ __device__ __forceinline__ void grad_store(const NormGradParams &p, size_t row, 
 
 // As the forward kernel; besides, every thread keeps the sums over its rows of dY h rstd for its columns.  At the end a workgroup
 // adds its row groups' sums in group order and leaves one row of partial sums in `work`: no atomics, the same sums every time.
+// Registers for four waves a SIMD up to 16 values a thread, two above: the grid is sized for that.
 template <typename T, int TPR, int CH>
-__global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_grad_kernel(const NormGradParams p)
+__global__ __launch_bounds__(TPR > NT ? TPR : NT, TPR > NT ? 4 : CH * vec_of<T>() <= 16 ? 4 : 2) void norm_grad_kernel(const NormGradParams p)
 {
     constexpr int N = vec_of<T>(), NTH = TPR > NT ? TPR : NT, RPW = NTH / TPR;
     __shared__ float sh[2 * (NTH / 64)];
@@ -512,31 +513,38 @@ __global__ __launch_bounds__(NT) void norm_grad_weight_kernel(const NormGradPara
     p.work[(size_t)blockIdx.y * p.cols + c] = s;
 }
 
-// dW[c] = sum of the groups' partial sums: 32 columns a workgroup, 8 threads of 4 columns; 32 such rows of threads take every 32nd group,
-// and their sums are added in order.
-__global__ __launch_bounds__(NT) void norm_grad_reduce_kernel(const float *work, float *dW, int cols, int groups)
+// dW[c] = sum of the groups' partial sums: 32 columns a workgroup, 8 threads of 4 columns; 128 such rows of threads take every 128th
+// group, so that all of a thread's loads are under way at once (the sums were written by other XCDs: each load goes to memory), and
+// their sums are added in order.
+__global__ __launch_bounds__(1024) void norm_grad_reduce_kernel(const float *work, float *dW, int cols, int groups)
 {
-    __shared__ float sh[32][33];
+    __shared__ float sh[128][33], sh2[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 7) * 4, k = threadIdx.x >> 3;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int g = k; g < groups; g += 32)
-    {
-        float v[4];
-        load_vals<float>(work + (size_t)g * cols + c, cols - c, v);
+    float v[ROWS_GRAD_MAX_WG / 128][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { s[i] += v[i]; }
+    for (int j = 0; j < ROWS_GRAD_MAX_WG / 128; ++j)
+    {
+        const int g = j * 128 + k;
+        load_vals<float>(work + (size_t)g * cols + c, g < groups ? cols - c : 0, v[j]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { sh[k][(threadIdx.x & 7) * 4 + i] = s[i]; }
-    __syncthreads();
-    const int d = blockIdx.x * 32 + threadIdx.x;
-    if (threadIdx.x < 32 && d < cols)
+    for (int i = 0; i < 4; ++i)
     {
-        float t = 0.0f;
+        float s = v[0][i];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) { t += sh[j][threadIdx.x]; }
-        dW[d] = t;
+        for (int j = 1; j < ROWS_GRAD_MAX_WG / 128; ++j) { s += v[j][i]; }
+        sh[k][(threadIdx.x & 7) * 4 + i] = s;
+    }
+    __syncthreads();
+    const int d = threadIdx.x & 31, q = threadIdx.x >> 5;
+    sh2[q][d] = ((sh[4 * q][d] + sh[4 * q + 1][d]) + sh[4 * q + 2][d]) + sh[4 * q + 3][d];
+    __syncthreads();
+    if (q == 0 && (int)blockIdx.x * 32 + d < cols)
+    {
+        float t = sh2[0][d];
+#pragma unroll
+        for (int j = 1; j < 32; ++j) { t += sh2[j][d]; }
+        dW[blockIdx.x * 32 + d] = t;
     }
 }
 
@@ -555,36 +563,49 @@ __device__ __forceinline__ void store_e4m3_16(uint8_t *q, int n, const float (&x
     }
 }
 
-// 8 lanes take a block of a row, 16 elements each; row and block move by fixed steps.
+// 16 lanes take a block of a row, 8 elements each, two blocks under way at a time; row and block move by fixed steps.
 template <typename T>
 __global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, size_t rows, int cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, int nb,
                                                       size_t step_row, int step_b)
 {
     constexpr int V = vec_of<T>();
-    const int l = threadIdx.x & 7;
-    const size_t first = (size_t)blockIdx.x * (NT / 8) + threadIdx.x / 8;
+    const int l = threadIdx.x & 15;
+    const size_t first = (size_t)blockIdx.x * (NT / 16) + threadIdx.x / 16;
     size_t row = first / (unsigned)nb;
     int b = (int)(first - row * (unsigned)nb);
     while (row < rows)
     {
-        const int c = b * ROWS_BLOCK + l * 16;
-        float x[16];
+        size_t rr[2];
+        int cc[2];
+        float x[2][8];
 #pragma unroll
-        for (int k = 0; k < 16; k += V)
+        for (int u = 0; u < 2; ++u)
         {
-            float v[V];
-            load_vals<float>(X + row * ldx + c + k, cols - c - k, v);
+            rr[u] = row; cc[u] = b * ROWS_BLOCK + l * 8;
 #pragma unroll
-            for (int i = 0; i < V; ++i) { x[k + i] = v[i]; }
+            for (int k = 0; k < 8; k += V)
+            {
+                float v[V];
+                load_vals<float>(X + row * ldx + cc[u] + k, row < rows ? cols - cc[u] - k : 0, v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) { x[u][k + i] = v[i]; }
+            }
+            row += step_row; b += step_b;
+            if (b >= nb) { b -= nb; ++row; }
         }
-        unsigned amax = 0u;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { amax = max(amax, finite_bits(x[i])); }
-        const unsigned e = block_exponent(lanes_max<8>(amax));
-        store_e4m3_16(Q + row * ldq + c, cols - c, x, block_factor(e));
-        if (l == 0) { S[row * lds + b] = (uint8_t)e; }
-        row += step_row; b += step_b;
-        if (b >= nb) { b -= nb; ++row; }
+        for (int u = 0; u < 2; ++u)
+        {
+            unsigned amax = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { amax = max(amax, finite_bits(x[u][i])); }
+            const unsigned e = block_exponent(lanes_max<16>(amax));
+            if (rr[u] < rows)
+            {
+                store_e4m3(Q + rr[u] * ldq + cc[u], cols - cc[u], x[u], block_factor(e));
+                if (l == 0) { S[rr[u] * lds + cc[u] / ROWS_BLOCK] = (uint8_t)e; }
+            }
+        }
     }
 }
 
@@ -684,7 +705,7 @@ void norm_grad_go(const NormGradParams &p, hipStream_t s)
     ROWS_BY_WIDTH(T, p.rows, p.cols, GO, WIDE);
 #undef WIDE
 #undef GO
-    if (p.dW) { hipLaunchKernelGGL(norm_grad_reduce_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(NT), 0, s, p.work, p.dW, p.cols, groups); }
+    if (p.dW) { hipLaunchKernelGGL(norm_grad_reduce_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(1024), 0, s, p.work, p.dW, p.cols, groups); }
 }
 
 template <typename T>
@@ -706,7 +727,7 @@ void quantize_go(size_t rows, size_t cols, const void *X, size_t ldx, uint8_t *Q
         hipLaunchKernelGGL(quantize_transpose_kernel<T>, dim3((unsigned)(nrb * ncb)), dim3(NT), 0, s, x, ldx, rows, cols, Q, ldq, S, lds, (unsigned)ncb);
         return;
     }
-    const size_t nb = (cols + ROWS_BLOCK - 1) / ROWS_BLOCK, want = (rows * nb + NT / 8 - 1) / (NT / 8), grid = want < 4096 ? want : 4096, width = grid * (NT / 8);
+    const size_t nb = (cols + ROWS_BLOCK - 1) / ROWS_BLOCK, want = (rows * nb + NT / 16 - 1) / (NT / 16), grid = want < 4096 ? want : 4096, width = grid * (NT / 16);
     hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)grid), dim3(NT), 0, s, x, ldx, rows, (int)cols, Q, ldq, S, lds, (int)nb, width / nb, (int)(width % nb));
 }
 

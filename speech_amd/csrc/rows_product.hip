@@ -180,15 +180,20 @@ __device__ __forceinline__ void load_dwords_to_lds_if(bool yes, const uint8_t *o
 
 //
 // STAGES stages are in LDS: one is read while the others arrive.  Scales go through LDS too, a dword of four k-steps for each row.
-template <typename T, int TM, int TN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
+//
+// GROUPS such sets of waves share a tile: each takes every GROUPS-th k-step into stages of its own, and their sums are added in the end.
+// With one group a SIMD has one wave, which waits for LDS, multiplies, waits; two fill each other's gaps where the tiles are few and K long.
+template <typename T, int TM, int TN, int WM, int WN, int STAGES, int GROUPS>
+__global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
 {
-    constexpr int NTH = 64 * WM * WN, MT = TM / WM / 16, NN = TN / WN / 16, ROWS = TM + TN, STAGE = ROWS * 128;
+    constexpr int NTH = 64 * WM * WN, MT = TM / WM / 16, NN = TN / WN / 16, ROWS = TM + TN, STAGE = ROWS * 128, SCALES = STAGES * STAGE, SET = SCALES + 2 * ROWS * 4;
     constexpr int LA = TM * 8 / NTH, LB = TN * 8 / NTH, LOADS = LA + LB;     // 16-byte loads a thread makes for a stage
     constexpr int LS = (ROWS + NTH - 1) / NTH;                               // and dwords for four stages' scales
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    uint8_t *lds_scales = lds + STAGES * STAGE;
-    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g = lane >> 4;
+    static_assert(GROUPS * SET >= NTH * MT * NN * 16, "the groups' sums are handed over in LDS");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t all_lds[];
+    const int group = GROUPS == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / NTH), tid = (int)threadIdx.x - group * NTH;
+    uint8_t *lds = all_lds + group * SET;
+    const int lane = tid & 63, l16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
 
     // XCDs take workgroups in turn: each gets a run of consecutive tiles, which walk 8 tiles of rows at a time so that the tiles an XCD
@@ -217,26 +222,28 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
     const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds);
     const int last = (int)(p.K - (size_t)(nb - 1) * 128);                    // bytes of the last k-step: 1 ... 128
 
-    // chunks that start at or behind K are fetched from the row's first bytes (they are cleared in LDS below)
-    auto fetch = [&](int kb)
+    // s counts the group's k-steps; chunks that start at or behind K are fetched from the row's first bytes (they are cleared in LDS below)
+    auto fetch = [&](int s)
     {
+        const int kb = s * GROUPS + group;
+        if (kb >= nb) { return; }
+        if (s % (4 / GROUPS) == 0)                                           // the first of the four k-steps whose scales share dwords
+        {
+#pragma unroll
+            for (int i = 0; i < LS; ++i)
+            {
+                const int r0 = i * NTH + wave * 64;
+                if (r0 < ROWS) { load_dword_to_lds((r0 < TM ? SA : SB) + (kb & ~3), os[i], base + (unsigned)(SCALES + (kb >> 2 & 1) * (ROWS * 4) + r0 * 4)); }
+            }
+        }
         const bool cut = kb == nb - 1 && last < 128;
         const unsigned da = cut && ca * 16 >= last ? (unsigned)(ca * 16) : 0u, db = cut && cb * 16 >= last ? (unsigned)(cb * 16) : 0u;
         const uint8_t *a = A + (size_t)kb * 128, *b = B + (size_t)kb * 128;
-        const unsigned dst = base + (unsigned)((kb % STAGES) * STAGE + wave * 1024);
+        const unsigned dst = base + (unsigned)((s % STAGES) * STAGE + wave * 1024);
 #pragma unroll
         for (int i = 0; i < LA; ++i) { load_to_lds(a, oa[i] - da, dst + (unsigned)(i * (NTH * 16))); }
 #pragma unroll
         for (int i = 0; i < LB; ++i) { load_to_lds(b, ob[i] - db, dst + (unsigned)(TM * 128 + i * (NTH * 16))); }
-    };
-    auto fetch_scales = [&](int kb)                                          // before a group of four's first stage
-    {
-#pragma unroll
-        for (int i = 0; i < LS; ++i)
-        {
-            const int r0 = i * NTH + wave * 64;
-            if (r0 < ROWS) { load_dword_to_lds((r0 < TM ? SA : SB) + kb, os[i], base + (unsigned)(STAGES * STAGE + (kb >> 2 & 1) * (ROWS * 4) + r0 * 4)); }
-        }
     };
 
     v4f acc[MT][NN];
@@ -250,39 +257,36 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
     const int place = (g ^ (l16 & 7)) * 16, arow = wm * (TM / WM) + l16, brow = wn * (TN / WN) + 8 * (l16 >> 2) + (l16 & 3);
     const int qa = arow * 128 + place, qb = (TM + brow) * 128 + place;
 
-    for (int kb = 0; kb < STAGES - 1 && kb < nb; ++kb)
-    {
-        if ((kb & 3) == 0) { fetch_scales(kb); }
-        fetch(kb);
-    }
-    for (int kb = 0; kb < nb; ++kb)
+    const int steps = (nb + GROUPS - 1) / GROUPS;                            // of the group that has the most
+    for (int s = 0; s < STAGES - 1; ++s) { fetch(s); }
+    for (int s = 0; s < steps; ++s)
     {
         // this wave's loads of the stage have arrived: the STAGES - 2 stages behind it may be on their way, near the end everything is
         // waited for; a barrier alone does not wait for loads into LDS
-        if (kb + STAGES - 1 <= nb) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * LOADS) : "memory"); }
+        const int kb = s * GROUPS + group;
+        if (kb + (STAGES - 2) * GROUPS < nb) { asm volatile("s_waitcnt vmcnt(%0)" : : "n"((STAGES - 2) * LOADS) : "memory"); }
         else { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
         __syncthreads();                                                     // the stage is in LDS, the one before it is free
-        uint8_t *st = lds + (kb % STAGES) * STAGE;
-        if (kb == nb - 1 && last < 128)
+        uint8_t *st = lds + (s % STAGES) * STAGE;
+        if (s == steps - 1 && last < 128)
         {
-            for (int r = tid; r < ROWS; r += NTH)
+            if (kb == nb - 1)
             {
-                const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
-                for (int c = last / 16; c < 8; ++c)
+                for (int r = tid; r < ROWS; r += NTH)
                 {
-                    uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
-                    *q = keep_bytes(*q, last - c * 16);
+                    const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
+                    for (int c = last / 16; c < 8; ++c)
+                    {
+                        uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
+                        *q = keep_bytes(*q, last - c * 16);
+                    }
                 }
             }
             __syncthreads();
         }
-        const int ahead = kb + STAGES - 1;
-        if (ahead < nb)
-        {
-            if ((ahead & 3) == 0) { fetch_scales(ahead); }
-            fetch(ahead);
-        }
-        const uint8_t *sc = lds_scales + (kb >> 2 & 1) * (ROWS * 4) + (kb & 3);
+        fetch(s + STAGES - 1);
+        if (GROUPS > 1 && kb >= nb) { continue; }
+        const uint8_t *sc = lds + SCALES + (kb >> 2 & 1) * (ROWS * 4) + (kb & 3);
         v8i fb[NN];
         int sb[NN];
 #pragma unroll
@@ -302,6 +306,34 @@ __global__ __launch_bounds__(64 * WM * WN) void product_tile_kernel(const Produc
 #pragma unroll
             for (int j = 0; j < NN; ++j) { acc[i][j] = mfma_scaled(fb[j], fa, acc[i][j], sb[j], sa); }
         }
+    }
+    if (GROUPS > 1)
+    {
+        v4f *sums = reinterpret_cast<v4f *>(all_lds);
+        for (int from = 1; from < GROUPS; ++from)
+        {
+            __syncthreads();
+            if (group == from)
+            {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                {
+#pragma unroll
+                    for (int j = 0; j < NN; ++j) { sums[(i * NN + j) * NTH + tid] = acc[i][j]; }
+                }
+            }
+            __syncthreads();
+            if (group == 0)
+            {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                {
+#pragma unroll
+                    for (int j = 0; j < NN; ++j) { acc[i][j] += sums[(i * NN + j) * NTH + tid]; }
+                }
+            }
+        }
+        if (group != 0) { return; }
     }
 
     const size_t n = n0 + (size_t)(wn * (TN / WN) + 8 * g);
@@ -564,15 +596,15 @@ hipError_t stream_go(const ProductParams &p, hipStream_t s)
     return hipSuccess;
 }
 
-template <typename T, int TM, int TN, int WM, int WN, int STAGES>
+template <typename T, int TM, int TN, int WM, int WN, int STAGES, int GROUPS = 1>
 hipError_t tile_go(const ProductParams &p, hipStream_t s)
 {
-    constexpr int LDS = STAGES * (TM + TN) * 128 + 2 * (TM + TN) * 4;
-    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<T, TM, TN, WM, WN, STAGES>);
+    constexpr int LDS = GROUPS * (STAGES * (TM + TN) * 128 + 2 * (TM + TN) * 4);
+    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<T, TM, TN, WM, WN, STAGES, GROUPS>);
     const hipError_t e = opt_in_lds_once(k, LDS);
     if (e != hipSuccess) { return e; }
     const unsigned tm = (unsigned)((p.M + TM - 1) / TM), tn = (unsigned)((p.N + TN - 1) / TN);
-    hipLaunchKernelGGL((product_tile_kernel<T, TM, TN, WM, WN, STAGES>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN), LDS, s, p, tm, tn);
+    hipLaunchKernelGGL((product_tile_kernel<T, TM, TN, WM, WN, STAGES, GROUPS>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN * GROUPS), LDS, s, p, tm, tn);
     return hipSuccess;
 }
 
@@ -588,11 +620,12 @@ size_t tiles(const ProductParams &p, size_t tm, size_t tn) { return ((p.M + tm -
 
 // Which kernel: the largest tile that still gives the 256 CUs about one each, since a value then costs the fewest operand bytes.
 // Measured, us (rows x columns x k): the chosen kernel / the next larger tile / the next smaller one
-//   stream 256 x 256   4096 x 4096 x 1024 (256 tiles)    24.3 / - / 26.0       2048 fewer columns (128 tiles, k 4096): 46.4, 128 x 128: 34.8
+//   stream 256 x 256   4096 x 4096 x 1024 (256 tiles)    24.3 / - / 26.0       4096 x 2048 x 4096 (128): 46.4, 128 x 128: 34.8
 //   128 x 128          7984 x 1024 x 2048 (504)          20.6 / 28.7 / 25.4    2048 x 2048 x 2048 (256): 15.9, 128 x 64: 14.0
 //   128 x 64           2048 x 1024 x 7984 (256)          35.4 / 55.0 / 42.7    1024 x 1024 x 1024 (128): 6.9, 64 x 64: 5.6
 //   64 x 64            1024 x 1024 x 1024 (256)          5.6 / 6.9 / 11.3      512 x 512 x 512 (64): 4.4, split 32 x 32: 3.9
-//   split 32 x 32      64 x 2048 x 2048 (128)            6.8 / 7.8 / 6.6
+//     two groups       512 x 1024 x 4096 (128)           10.6, one group: 12.8     31936 x 512 x 720 (4000): 65, one group: 34
+//   split 32 x 32      64 x 2048 x 2048 (128)            6.8 / 7.8 / 6.6       300 x 1024 x 8192 (320): 44, 64 x 64 in two groups: 17.8
 //   split 16 x 16      1 x 8192 x 8192                   15.2 (4.4 TB/s of weights) / 19.2
 template <typename T>
 hipError_t product_go(const ProductParams &p, hipStream_t s)
@@ -603,6 +636,7 @@ hipError_t product_go(const ProductParams &p, hipStream_t s)
     if (near && p.M >= 256 && p.N >= 256 && p.K > 384 && tiles(p, 256, 256) >= 240) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
     if (near && tiles(p, 128, 128) >= 384) { return tile_go<T, 128, 128, 2, 2, 2>(p, s); }
     if (near && tiles(p, 128, 64) >= 192) { return tile_go<T, 128, 64, 2, 2, 3>(p, s); }
+    if (near && tiles(p, 64, 64) >= 64 && p.K >= 1024) { return tile_go<T, 64, 64, 2, 2, 3, 2>(p, s); }
     if (near && tiles(p, 64, 64) >= 160) { return tile_go<T, 64, 64, 2, 2, 3>(p, s); }
     return split_go<T, 2, 2, 8>(p, s);
 }
