@@ -255,7 +255,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(con
     }
     // row 16 i + l16 of A: chunk g ^ (l16 & 7); row 32 (j / 2) + 4 (j % 2) + 8 (l16 / 4) + l16 % 4 of B: the same
     const int place = (g ^ (l16 & 7)) * 16, arow = wm * (TM / WM) + l16, brow = wn * (TN / WN) + 8 * (l16 >> 2) + (l16 & 3);
-    const int qa = arow * 128 + place, qb = (TM + brow) * 128 + place;
+    int qa = arow * 128 + place, qb = (TM + brow) * 128 + place;
 
     const int steps = (nb + GROUPS - 1) / GROUPS;                            // of the group that has the most
     for (int s = 0; s < STAGES - 1; ++s) { fetch(s); }
@@ -377,6 +377,10 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(con
 // writing of the results stands between two tiles.  The last tiles of rows and columns are moved back to end with the matrix, so that no
 // tile has an edge (what two tiles share they compute alike).  M and N are at least 256, K more than 384 (four k-steps).
 // TAIL: K is no multiple of 128.
+//
+// Bound by the matrix units at the clock that the power limit leaves (they are busy 70 % of the cycles at about 1.8 GHz; with fewer waits the
+// clock falls and the time stays).  Measured, random values: 8192 x 8192 x 8192 in 396 ... 466 us from card to card (2.4 ... 2.8 PFLOP/s),
+// 8192 x 8192 x 8000 432 us beside 466 (rows of 8192 bytes meet in the same channels), 31936 x 4096 x 2048 251 us.
 template <typename T, bool TAIL>
 __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
 {
@@ -402,6 +406,11 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
     const int lr = tid >> 3, ca = (tid & 7) ^ swizzle_a(lr), cb = (tid & 7) ^ swizzle_b(lr);
     const unsigned stepa = 32u * (unsigned)p.lda, stepb = 32u * (unsigned)p.ldb;
     const unsigned oa = (unsigned)lr * (unsigned)p.lda + (unsigned)(ca * 16), ob = (unsigned)lr * (unsigned)p.ldb + (unsigned)(cb * 16);
+    // TAIL: the last k-step, which is not full, comes first of a tile.  Its chunks that start at or behind K are fetched from its first
+    // bytes, and what lies behind K is cleared in LDS between two tiles, where a branch and a barrier cost little (cleared in the middle of
+    // the stream, 8192 x 8192 x 8000 took 539 us instead of 432).
+    const unsigned oa_cut = (unsigned)lr * (unsigned)p.lda + (ca * 16 >= last ? 0u : (unsigned)(ca * 16)), ob_cut = (unsigned)lr * (unsigned)p.ldb + (cb * 16 >= last ? 0u : (unsigned)(cb * 16));
+    const size_t whole = TAIL ? (size_t)(nb - 1) * 128 : 0;
     const unsigned osa = (unsigned)tid * (unsigned)p.ldsa, osb = (unsigned)tid * (unsigned)p.ldsb;
     const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds);
     const unsigned lds0 = base + (unsigned)wave * 1024u, sc0 = base + SCALES + (unsigned)wave * 256u;
@@ -433,7 +442,7 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
     int sa[MT], sb[NN];
     // row 16 i + l16 of A: chunk g ^ (l16 & 7); row 32 (j / 2) + 4 (j % 2) + 8 (l16 / 4) + l16 % 4 of B: the same
     const int place = (g ^ (l16 & 7)) * 16, brow = wn * 128 + 8 * (l16 >> 2) + (l16 & 3), arow = wm * 128 + l16;
-    const int qa = arow * 128 + place, qb = TM * 128 + brow * 128 + place, qsa = SCALES + arow * 4, qsb = SCALES + (TM + brow) * 4;
+    int qa = arow * 128 + place, qb = TM * 128 + brow * 128 + place, qsa = SCALES + arow * 4, qsb = SCALES + (TM + brow) * 4;
     unsigned stage = 0, scales = 0;                                          // of the step that is read; scales: its byte among four as well
     auto read_a = [&](int i)
     {
@@ -457,21 +466,42 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
     auto look_ahead = [&]()
     {
         corner(tile + stride < end ? tile + stride : tile, mx, nx);
-        nA = p.A + mx * p.lda; nB = p.B + nx * p.ldb; nSA = p.SA + mx * p.ldsa; nSB = p.SB + nx * p.ldsb;
+        nA = p.A + mx * p.lda + whole; nB = p.B + nx * p.ldb + whole; nSA = p.SA + mx * p.ldsa; nSB = p.SB + nx * p.ldsb;
+    };
+    auto clear = [&]()
+    {
+        uint8_t *st = lds + stage;
+        for (int r = tid; r < TM + TN; r += 256)
+        {
+            const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
+            for (int c = last / 16; c < 8; ++c)
+            {
+                uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
+                *q = keep_bytes(*q, last - c * 16);
+            }
+        }
+        wait_read();
+        barrier();
+    };
+    auto first_operands = [&]()
+    {
+#pragma unroll
+        for (int j = 0; j < NN; ++j) { read_b(j); }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { read_a(i); }
     };
     corner(tile, m0, n0);
-    A = p.A + m0 * p.lda; B = p.B + n0 * p.ldb; SA = p.SA + m0 * p.ldsa; SB = p.SB + n0 * p.ldsb;
-    fetch_scales(0, true);
-    for_each<16>([&](auto i) { fetch(i, oa, ob); });
+    A = p.A + m0 * p.lda + whole; B = p.B + n0 * p.ldb + whole; SA = p.SA + m0 * p.ldsa; SB = p.SB + n0 * p.ldsb;
+    fetch_scales(TAIL ? nb - 1 & ~3 : 0, true);
+    for_each<16>([&](auto i) { fetch(i, TAIL ? oa_cut : oa, TAIL ? ob_cut : ob); });
     fstage ^= (unsigned)STAGE;
-    A += 128; B += 128;
+    if (TAIL) { A -= whole; B -= whole; fetch_scales(0, true); scales = (unsigned)(nb - 1 & 3); }
+    else { A += 128; B += 128; }
     for_each<16>([&](auto i) { fetch(i, oa, ob); });
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     barrier();
-#pragma unroll
-    for (int j = 0; j < NN; ++j) { read_b(j); }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { read_a(i); }
+    if (TAIL) { clear(); }
+    first_operands();
     look_ahead();
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -481,8 +511,8 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
     }
 
     // Between two matrix instructions there is room for the issue of about six others: what else a step has to do is handed out to its 2 x
-    // 32 places, and kept there; without TAIL a step is one run of instructions without a branch, across which the compiler would move
-    // them.  Place m of a half: column tile m / 4, row tile m % 4 (+ 4).
+    // 32 places, and kept there; a step is one run of instructions without a branch, across which the compiler would move them.
+    // Place m of a half: column tile m / 4, row tile m % 4 (+ 4).
     auto multiply = [&](int i, int j)
     {
         acc[i][j] = mfma_scaled(fb[j], fa[i], acc[i][j], sb[j], sa[i]);
@@ -492,7 +522,9 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
     {
         for (int k = 0; k < nb; ++k)                                         // k-step k + 2 is asked for, which for the last two is the next tile's
         {
+            if (TAIL) { asm volatile("" : "+s"(k)); }                        // one loop for all k: copies of it for the last ones would not agree on registers
             unsigned fo = oa, go = ob;
+            asm volatile("" : "+v"(fo), "+v"(go), "+v"(qa), "+v"(qb));       // 14 sums with row steps, kept over the loop, would push out other registers
             for_each<32>([&](auto mm)
             {
                 constexpr int m = decltype(mm)::value;
@@ -504,17 +536,23 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
                     fstage ^= (unsigned)STAGE;
                     const bool next = k == nb - 2;
                     A = next ? nA : A + 128; B = next ? nB : B + 128;
-                    if (TAIL)                                                    // chunks that start at or behind K come from the row's first bytes
+                    if (TAIL)
                     {
-                        fo -= k == nb - 3 && ca * 16 >= last ? (unsigned)(ca * 16) : 0u;
-                        go -= k == nb - 3 && cb * 16 >= last ? (unsigned)(cb * 16) : 0u;
+                        const size_t back = (whole + 128) & (0 - (size_t)(k == nb - 1));
+                        A -= back; B -= back;
+                        fo = next ? oa_cut : oa; go = next ? ob_cut : ob;
                     }
                 }
                 if (m == 12)
                 {
                     const bool next = k == nb - 2;
                     SA = next ? nSA : SA; SB = next ? nSB : SB;
-                    fetch_scales(next ? 0 : k + 2, next || ((k & 3) == 2 && k < nb - 2));
+                    if (TAIL)
+                    {
+                        const int is_next = -(int)next, is_last = -(int)(k == nb - 1);
+                        fetch_scales((nb - 1 & ~3 & is_next) | (k + 1 & ~(is_next | is_last)), next | (k == nb - 1) | (((k & 3) == 3) & (k < nb - 2)));
+                    }
+                    else { fetch_scales(next ? 0 : k + 2, next || ((k & 3) == 2 && k < nb - 2)); }
                 }
                 if constexpr (m >= 9 && m % 4 == 1) { fetch(std::integral_constant<int, (m - 9) / 4>(), fo, go); }
                 multiply(m % 4, m / 4);
@@ -525,25 +563,12 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
             barrier();                                                           // the next stage is there
             stage ^= (unsigned)STAGE;
             // the next step's scale byte; behind a group of four or the tile, the other buffer's first
-            scales = k == nb - 1 || (k & 3) == 3 ? (scales & 2048u) ^ 2048u : scales + 1u;
             if (TAIL)
             {
-                if (k == nb - 2)
-                {
-                    uint8_t *st = lds + stage;
-                    for (int r = tid; r < TM + TN; r += 256)
-                    {
-                        const int f = r < TM ? swizzle_a(r) : swizzle_b(r - TM);
-                        for (int c = last / 16; c < 8; ++c)
-                        {
-                            uint4 *q = reinterpret_cast<uint4 *>(st + r * 128 + ((c ^ f) * 16));
-                            *q = keep_bytes(*q, last - c * 16);
-                        }
-                    }
-                    wait_read();
-                    barrier();
-                }
+                const unsigned is_last = 0u - (unsigned)(k == nb - 1), other = 0u - (unsigned)((k == nb - 1) | ((k & 3) == 0));
+                scales = ((((scales & 2048u) ^ 2048u) + ((unsigned)(nb - 1 & 3) & is_last)) & other) | (scales + 1u & ~other);
             }
+            else { scales = k == nb - 1 || (k & 3) == 3 ? (scales & 2048u) ^ 2048u : scales + 1u; }
             for_each<32>([&](auto mm)
             {
                 constexpr int m = decltype(mm)::value;
@@ -561,26 +586,34 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
         int row = arow, col = wn * 128 + 8 * g;
         asm volatile("" : "+s"(ldy), "+v"(row), "+v"(col));
         const size_t n = n0 + (size_t)col;
+        float bias[NN / 2][8] = {};
+        if (p.bias)                                                          // all before the first store, so that none waits for another
+        {
+#pragma unroll
+            for (int h = 0; h < NN / 2; ++h) { load_bias(p.bias + n + 32 * h, bias[h]); }
+        }
 #pragma unroll
         for (int h = 0; h < NN / 2; ++h)
         {
             T *y = reinterpret_cast<T *>(p.Y) + (m0 + (size_t)row) * ldy + n + 32 * h;
-            float bias[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            if (p.bias) { load_bias(p.bias + n + 32 * h, bias); }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
             {
                 float v[8];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) { v[q] = acc[i][2 * h + q / 4][q % 4] + bias[q]; acc[i][2 * h + q / 4][q % 4] = 0.0f; }
+                for (int q = 0; q < 8; ++q) { v[q] = acc[i][2 * h + q / 4][q % 4] + bias[h][q]; acc[i][2 * h + q / 4][q % 4] = 0.0f; }
                 store_vals(y, 8, v);
                 y += 16 * ldy;
+                asm volatile("" : "+v"(y));
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         tile += stride;
         if (tile >= end) { break; }
         m0 = mx; n0 = nx;
         look_ahead();
+        if (TAIL) { clear(); }
+        first_operands();                                                    // once more, so that their registers are free while the results are written
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");                       // the loads behind the last tile, before its LDS is another's
 }
