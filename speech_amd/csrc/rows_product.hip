@@ -651,26 +651,35 @@ hipError_t split_go(const ProductParams &p, hipStream_t s)
 
 size_t tiles(const ProductParams &p, size_t tm, size_t tn) { return ((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn); }
 
-// Which kernel: the largest tile that still gives the 256 CUs about one each, since a value then costs the fewest operand bytes.
-// Measured, us (rows x columns x k): the chosen kernel / the next larger tile / the next smaller one
-//   stream 256 x 256   4096 x 4096 x 1024 (256 tiles)    24.3 / - / 26.0       4096 x 2048 x 4096 (128): 46.4, 128 x 128: 34.8
-//   128 x 128          7984 x 1024 x 2048 (504)          20.6 / 28.7 / 25.4    2048 x 2048 x 2048 (256): 15.9, 128 x 64: 14.0
-//   128 x 64           2048 x 1024 x 7984 (256)          35.4 / 55.0 / 42.7    1024 x 1024 x 1024 (128): 6.9, 64 x 64: 5.6
-//   64 x 64            1024 x 1024 x 1024 (256)          5.6 / 6.9 / 11.3      512 x 512 x 512 (64): 4.4, split 32 x 32: 3.9
-//     two groups       512 x 1024 x 4096 (128)           10.6, one group: 12.8     31936 x 512 x 720 (4000): 65, one group: 34
-//   split 32 x 32      64 x 2048 x 2048 (128)            6.8 / 7.8 / 6.6       300 x 1024 x 8192 (320): 44, 64 x 64 in two groups: 17.8
-//   split 16 x 16      1 x 8192 x 8192                   15.2 (4.4 TB/s of weights) / 19.2
+// Which kernel: the largest tile whose last round over the 256 CUs is not mostly empty, since a value then costs the fewest operand bytes.
+// A CU holds one workgroup of 256 x 256, two of 128 x 128 or 128 x 64, three of 64 x 64.  Measured, us:
+//                        256 x 256   128 x 128   128 x 64   64 x 64   64 x 64, K in two   32 x 32, K in eight
+//   31936 x 4096 x 720       138 *       183         218        234
+//   4096 x 4096 x 2048        37 *        43          60         67
+//   4096 x 4096 x 512         19          17 *        21         22
+//   4300 x 4300 x 2048        59          48 *        57         64       289 tiles of 256 x 256 are two rounds
+//   2304 x 2048 x 2048        27          17 *        21         19       576 tiles of 128 x 64 are two rounds of two a CU
+//   2048 x 2048 x 2048        27          15          13 *       17
+//   2048 x 1024 x 7984        84          55          34 *       40       45
+//   2048 x 1024 x 2048        25          14          10.8       9.8 *    13
+//   1400 x 1024 x 2048        25          14          10.6       9.5 *    12.6
+//   1000 x 900 x 2048         25          14          10.3       8.3      7.3 *               20
+//   384 x 1024 x 1024         17          8.9         6.8        6.2      5.1 *               6.5
+//   256 x 512 x 2048          25          13          10         8.0      6.7                 6.7 *
+//   98 x 2048 x 1024                      8.8         6.7        5.3      5.3                 4.9 *
 template <typename T>
 hipError_t product_go(const ProductParams &p, hipStream_t s)
 {
     if (p.M <= 16) { return p.K <= 1024 ? split_go<T, 1, 1, 8>(p, s) : split_go<T, 1, 1, 16>(p, s); }      // 16 k-steps give 16 waves one each
     // rows of a tile are addressed in 32 bits from its first
     const bool near = p.K > 0 && p.lda < ((size_t)1 << 23) && p.ldb < ((size_t)1 << 23) && p.ldsa < ((size_t)1 << 23) && p.ldsb < ((size_t)1 << 23);
-    if (near && p.M >= 256 && p.N >= 256 && p.K > 384 && tiles(p, 256, 256) >= 240) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
-    if (near && tiles(p, 128, 128) >= 384) { return tile_go<T, 128, 128, 2, 2, 2>(p, s); }
-    if (near && tiles(p, 128, 64) >= 192) { return tile_go<T, 128, 64, 2, 2, 3>(p, s); }
-    if (near && tiles(p, 64, 64) >= 64 && p.K >= 1024) { return tile_go<T, 64, 64, 2, 2, 3, 2>(p, s); }
-    if (near && tiles(p, 64, 64) >= 160) { return tile_go<T, 64, 64, 2, 2, 3>(p, s); }
+    const size_t t256 = tiles(p, 256, 256), rounds = (t256 + 255) / 256, t64 = tiles(p, 64, 64);
+    const bool full = 5 * t256 >= 4 * 256 * rounds, amortized = p.K > 512 || (p.K > 384 && rounds > 1);
+    if (near && p.M >= 256 && p.N >= 256 && full && amortized) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
+    if (near && tiles(p, 128, 64) > 512) { return tile_go<T, 128, 128, 2, 2, 2>(p, s); }
+    if (near && (t64 > 768 || (t64 > 256 && p.K > 4096))) { return tile_go<T, 128, 64, 2, 2, 3>(p, s); }
+    if (near && t64 > 256) { return tile_go<T, 64, 64, 2, 2, 3>(p, s); }
+    if (near && t64 * p.K > 65536) { return tile_go<T, 64, 64, 2, 2, 3, 2>(p, s); }
     return split_go<T, 2, 2, 8>(p, s);
 }
 
