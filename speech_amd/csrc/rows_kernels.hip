@@ -610,13 +610,17 @@ __global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, si
 }
 
 // The transpose's form: a workgroup reads 128 rows of 64 columns into LDS and writes 64 rows of one block; 8 threads take a column,
-// 16 of its values each.  Rows of LDS are 65 words, so that neither the writing of rows nor the reading of columns piles up on banks.
+// 16 of its values each.  Rows of LDS are a word longer, so that neither the writing of rows nor the reading of columns piles up on banks;
+// they hold the values in their own type, so that 8 workgroups of 16-bit values fit a CU (as floats 4).
 constexpr int QT_COLS = 64;
 template <typename T>
 __global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size_t ldx, size_t rows, size_t cols, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds, unsigned ncb)
 {
     constexpr int V = vec_of<T>(), VR = QT_COLS / V;                         // vectors of a row
-    __shared__ float sh[ROWS_BLOCK * (QT_COLS + 1)];
+    constexpr int W = 4 / (int)sizeof(T), ROW = QT_COLS + W;                 // values of a word; of a row
+    typedef T Word __attribute__((ext_vector_type(W)));
+    __shared__ Word words[ROWS_BLOCK * ROW / W];
+    const T *sh = reinterpret_cast<const T *>(words);
     const unsigned rb = blockIdx.x / ncb;
     const size_t r0 = (size_t)rb * ROWS_BLOCK, c0 = (size_t)(blockIdx.x - rb * ncb) * QT_COLS;
     const int rleft = (int)min(rows - r0, (size_t)ROWS_BLOCK), cleft = (int)min(cols - c0, (size_t)QT_COLS);
@@ -632,7 +636,13 @@ __global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size
     {
         const int i = k * NT + threadIdx.x, r = i / VR, c = (i % VR) * V;
 #pragma unroll
-        for (int j = 0; j < V; ++j) { sh[r * (QT_COLS + 1) + c + j] = v[k][j]; }
+        for (int j = 0; j < V; j += W)
+        {
+            Word w;
+#pragma unroll
+            for (int q = 0; q < W; ++q) { w[q] = (T)v[k][j + q]; }
+            words[(r * ROW + c + j) / W] = w;
+        }
     }
     __syncthreads();
     const int g = threadIdx.x % 8;
@@ -643,7 +653,7 @@ __global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size
         float x[16];
         unsigned amax = 0u;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { x[i] = sh[(g * 16 + i) * (QT_COLS + 1) + c]; amax = max(amax, finite_bits(x[i])); }
+        for (int i = 0; i < 16; ++i) { x[i] = (float)sh[(g * 16 + i) * ROW + c]; amax = max(amax, finite_bits(x[i])); }
         const unsigned e = block_exponent(lanes_max<8>(amax));
         if (c >= cleft) { continue; }
         store_e4m3_16(Q + (c0 + c) * ldq + r0 + g * 16, rleft - g * 16, x, block_factor(e));
