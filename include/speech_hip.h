@@ -292,10 +292,15 @@ int speech_rows_quantize(int device, int dtype, size_t rows, size_t cols, const 
    is usually kept), summed in 32-bit floats and rounded once to dtype: SPEECH_BF16 or SPEECH_F16.  bias: NULL, or cols floats.
    k == 0 gives the bias.  The matrix unit adds each eight products (columns 8 i ... 8 i + 7) at a resolution of 2^-13 of the largest of
    them before they join the 32-bit sum: 1e-5 ... 4e-5 of a result as matrices of activations and weights have them, a tenth of a
-   16-bit type's own rounding, but no 32-bit result; there is none. */
+   16-bit type's own rounding, but no 32-bit result; there is none.
+   work: NULL, or work_bytes of device memory on 16 bytes that no other call in flight uses (two captured graphs that may run at once need
+   one each).  With as much as speech_rows_product_work gives (0 for most sizes), a product of few values over a long k, like the gradient of
+   a small layer's weights over many frames, is split over k; with less it is computed whole, which gives the same but for the order of its
+   32-bit sums. */
 int speech_rows_product(int device, int dtype, size_t rows, size_t cols, size_t k, const unsigned char *A, size_t lda,
                         const unsigned char *SA, size_t ldsa, const unsigned char *B, size_t ldb, const unsigned char *SB, size_t ldsb,
-                        const float *bias, void *Y, size_t ldy, void *stream);
+                        const float *bias, void *Y, size_t ldy, void *work, size_t work_bytes, void *stream);
+int speech_rows_product_work(size_t rows, size_t cols, size_t k, size_t *bytes);
 
 #ifdef __cplusplus
 }

@@ -26,7 +26,7 @@ EXT_SYMBOLS = [
     "speech_batch_splice_subsample", "speech_batch_subsample_rows", "speech_extract_pcm16", "speech_batch_set_ids", "speech_plan_run_host", "speech_host_release",
     "speech_batch_cmvn_noalloc", "speech_run_host_multi", "speech_shard_utterances", "speech_opts_frames", "speech_set_dropin_dither", "speech_batch_synth_audio", "speech_synth_audio_host",
     "speech_batch_row_keys", "speech_rows_dropout", "speech_rows_rms_norm", "speech_rows_rms_norm_backward", "speech_rows_rms_norm_work",
-    "speech_rows_quantize", "speech_rows_product",
+    "speech_rows_quantize", "speech_rows_product", "speech_rows_product_work",
 ]
 
 
@@ -138,7 +138,8 @@ def load():
     lib.speech_rows_rms_norm_backward.argtypes = [i, C.POINTER(SpeechNormGrad), vp]; lib.speech_rows_rms_norm_backward.restype = i
     lib.speech_rows_rms_norm_work.argtypes = [z, z, pz]; lib.speech_rows_rms_norm_work.restype = i
     lib.speech_rows_quantize.argtypes = [i, i, z, z, vp, z, vp, z, vp, z, i, vp]; lib.speech_rows_quantize.restype = i
-    lib.speech_rows_product.argtypes = [i, i, z, z, z, vp, z, vp, z, vp, z, vp, z, vp, vp, z, vp]; lib.speech_rows_product.restype = i
+    lib.speech_rows_product.argtypes = [i, i, z, z, z, vp, z, vp, z, vp, z, vp, z, vp, vp, z, vp, z, vp]; lib.speech_rows_product.restype = i
+    lib.speech_rows_product_work.argtypes = [z, z, z, pz]; lib.speech_rows_product_work.restype = i
     _lib = lib
     return lib
 

@@ -504,10 +504,10 @@ def _rows_check(rc):
 
 def held(rows, cols, device="cuda"):
     """(Q, S): room for a rows x cols matrix in 8-bit form, with the padding that the operators need: e4m3 values whose rows start on
-    16 bytes, and a scale byte for each block of 128 columns, rows of them on 4 bytes"""
+    16 bytes (long ones on 128, which product reads faster), and a scale byte for each block of 128 columns, rows of them on 4 bytes"""
     import torch
-    nb = -(-cols // 128)
-    q = torch.zeros(rows, -(-cols // 16) * 16, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
+    nb, pad = -(-cols // 128), 16 if cols < 512 else 128
+    q = torch.zeros(rows, -(-cols // pad) * pad, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
     return q, torch.zeros(rows, -(-nb // 4) * 4, dtype=torch.uint8, device=device)[:, :nb]
 
 
@@ -600,9 +600,16 @@ def quantize(X, Q, S, transpose=False, stream=None):
     _rows_check(types.lib.speech_rows_quantize(dev, code, rows, cols, xp, ldx, qp, ldq, sp, lds, 1 if transpose else 0, stream))
 
 
-def product(A, SA, B, SB, Y, bias=None, stream=None):
+def product_work(rows, cols, k):
+    """bytes of `work` that let product split a long k where there are few values; 0 where there is nothing to gain"""
+    n = C.c_size_t()
+    _rows_check(_lib.load().speech_rows_product_work(int(rows), int(cols), int(k), C.byref(n)))
+    return n.value
+
+
+def product(A, SA, B, SB, Y, bias=None, work=None, stream=None):
     """Y = A B^T + bias for A (rows x k) and B (columns x k, a weight matrix with a row for each output) in 8-bit form; Y bfloat16 or
-    float16, bias float32"""
+    float16, bias float32.  work: None, or a uint8 tensor of product_work(rows, cols, k) bytes, not used by another call in flight"""
     types, code, same, dev = _rows(Y, "Y")                     # float32 is refused by the C side
     rows, cols = Y.shape
     k = A.shape[1]
@@ -612,8 +619,9 @@ def product(A, SA, B, SB, Y, bias=None, stream=None):
     bp, ldb = _rows_arg(B, "B", dev, types.held, cols, k, 16)
     sb, ldsb = _rows_arg(SB, "SB", dev, types.scales, cols, nb, 4)
     yp, ldy = _rows_arg(Y, "Y", dev, same, rows, cols)
+    wp, wn = (None, 0) if work is None else (_vector_arg(work, "work", dev, types.bytes, work.numel()), work.numel())
     _rows_check(types.lib.speech_rows_product(dev, code, rows, cols, k, ap, lda, sa, ldsa, bp, ldb, sb, ldsb,
-                                              None if bias is None else _vector_arg(bias, "bias", dev, (types.f32,), cols), yp, ldy, stream))
+                                              None if bias is None else _vector_arg(bias, "bias", dev, (types.f32,), cols), yp, ldy, wp, wn, stream))
 
 
 def merge_stats(s, q, n, group=None):

@@ -206,9 +206,18 @@ int speech_rows_quantize(int device, int dtype, size_t rows, size_t cols, const 
     return 0;
 }
 
+int speech_rows_product_work(size_t rows, size_t cols, size_t k, size_t *bytes)
+{
+    const char *fn = "speech_rows_product_work";
+    if (!bytes) { return fail(fn, "null pointer bytes"); }
+    if (check_sizes(fn, rows, cols) || check_sizes(fn, rows, k)) { return 1; }
+    *bytes = rows && cols ? rows_product_work(rows, cols, k) : 0;
+    return 0;
+}
+
 int speech_rows_product(int device, int dtype, size_t rows, size_t cols, size_t k, const unsigned char *A, size_t lda,
                         const unsigned char *SA, size_t ldsa, const unsigned char *B, size_t ldb, const unsigned char *SB, size_t ldsb,
-                        const float *bias, void *Y, size_t ldy, void *stream)
+                        const float *bias, void *Y, size_t ldy, void *work, size_t work_bytes, void *stream)
 {
     const char *fn = "speech_rows_product";
     if (dtype != SPEECH_BF16 && dtype != SPEECH_F16) { return fail(fn, "dtype %d: the result has 16 bits (bf16 or f16)", dtype); }
@@ -218,9 +227,10 @@ int speech_rows_product(int device, int dtype, size_t rows, size_t cols, size_t 
     if (check_rows(fn, "Y", Y, ldy, cols, elem_of(dtype))) { return 1; }
     if ((uintptr_t)bias % 4u) { return fail(fn, "bias is not aligned to its elements"); }
     if (((rows + 15) / 16) * ((cols + 15) / 16) > MAX_GRID) { return fail(fn, "matrix too large"); }
+    if ((uintptr_t)work % 16u) { return fail(fn, "work must start on 16 bytes"); }
     OnDevice g(device);
     if (!g.ok) { return fail(fn, "cannot select device %d", device); }
-    const ProductParams p{rows, cols, k, A, SA, B, SB, lda, ldsa, ldb, ldsb, bias, Y, ldy};
+    const ProductParams p{rows, cols, k, A, SA, B, SB, lda, ldsa, ldb, ldsb, bias, Y, ldy, (float *)work, work ? work_bytes : 0, 0};
     HIP_TRY(fn, launch_rows_product(dtype, p, (hipStream_t)stream));
     return 0;
 }

@@ -46,6 +46,9 @@ struct ProductParams {
     const float *bias;
     void *Y;
     size_t ldy;
+    float *work;
+    size_t work_bytes;
+    size_t part;                                                             // columns of a part where k is split
 };
 
 hipError_t launch_row_keys(const UttDesc *utts, uint32_t nutt, const TileDesc *tiles, uint32_t ntiles, int n, int offset,
@@ -55,6 +58,7 @@ hipError_t launch_rows_norm(int dtype, const NormParams &p, hipStream_t s);
 hipError_t launch_rows_norm_grad(int dtype, const NormGradParams &p, hipStream_t s);
 hipError_t launch_rows_quantize(int dtype, size_t rows, size_t cols, const void *X, size_t ldx, uint8_t *Q, size_t ldq, uint8_t *S, size_t lds,
                                 int transpose, hipStream_t s);
+size_t rows_product_work(size_t M, size_t N, size_t K);
 hipError_t launch_rows_product(int dtype, const ProductParams &p, hipStream_t s);
 
 #if defined(__HIPCC__)

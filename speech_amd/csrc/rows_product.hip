@@ -187,8 +187,11 @@ __device__ __forceinline__ void load_dwords_to_lds_if(bool yes, const uint8_t *o
 //
 // GROUPS such sets of waves share a tile: each takes every GROUPS-th k-step into stages of its own, and their sums are added in the end.
 // With one group a SIMD has one wave, which waits for LDS, multiplies, waits; two fill each other's gaps where the tiles are few and K long.
-template <typename T, int TM, int TN, int WM, int WN, int STAGES, int GROUPS>
-__global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n)
+//
+// PARTS: the k-steps are split into `parts` ranges of p.part columns (a multiple of 512: four k-steps share dwords of scales), each another
+// workgroup's; T is float, and a part leaves its sums, M x N of them, in p.work.
+template <typename T, int TM, int TN, int WM, int WN, int STAGES, int GROUPS, bool PARTS>
+__global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(const ProductParams p, unsigned tiles_m, unsigned tiles_n, unsigned parts)
 {
     constexpr int NTH = 64 * WM * WN, MT = TM / WM / 16, NN = TN / WN / 16, ROWS = TM + TN, STAGE = ROWS * 128, SCALES = STAGES * STAGE, SET = SCALES + 2 * ROWS * 4;
     constexpr int LA = TM * 8 / NTH, LB = TN * 8 / NTH, LOADS = LA + LB;     // 16-byte loads a thread makes for a stage
@@ -202,15 +205,17 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(con
 
     // XCDs take workgroups in turn: each gets a run of consecutive tiles, which walk 8 tiles of rows at a time so that the tiles an XCD
     // works on share their rows of A and B in its L2
-    const unsigned total = tiles_m * tiles_n, per = (total + 7) / 8;
-    const unsigned tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || tile >= total) { return; }
+    const unsigned tiles = tiles_m * tiles_n, total = PARTS ? tiles * parts : tiles, per = (total + 7) / 8;
+    const unsigned at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || at >= total) { return; }
+    const unsigned part = PARTS ? at / tiles : 0u, tile = at - part * tiles;  // an XCD's tiles are of few parts, whose operands it reads once
     const unsigned band = tile / (8 * tiles_n), in = tile - band * 8 * tiles_n, bh = min(8u, tiles_m - band * 8);
     const size_t m0 = (size_t)(band * 8 + in % bh) * TM, n0 = (size_t)(in / bh) * TN;
 
-    const int nb = (int)((p.K + 127) / 128);
+    const size_t k0 = PARTS ? part * p.part : 0, K = PARTS ? min(p.K - k0, p.part) : p.K;
+    const int nb = (int)((K + 127) / 128);
     const int am = (int)min(p.M - m0, (size_t)TM) - 1, bm = (int)min(p.N - n0, (size_t)TN) - 1;     // last row of the tile that exists
-    const uint8_t *A = p.A + m0 * p.lda, *B = p.B + n0 * p.ldb, *SA = p.SA + m0 * p.ldsa, *SB = p.SB + n0 * p.ldsb;
+    const uint8_t *A = p.A + m0 * p.lda + k0, *B = p.B + n0 * p.ldb + k0, *SA = p.SA + m0 * p.ldsa + k0 / 128, *SB = p.SB + n0 * p.ldsb + k0 / 128;
     const int lr = tid >> 3, ca = (tid & 7) ^ swizzle_a(lr), cb = (tid & 7) ^ swizzle_b(lr);         // NTH / 8 rows a load, a multiple of 16
     unsigned oa[LA], ob[LB], os[LS];
 #pragma unroll
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(con
         os[i] = r < TM ? (unsigned)min(r, am) * (unsigned)p.ldsa : (unsigned)min(r - TM, bm) * (unsigned)p.ldsb;
     }
     const unsigned base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds);
-    const int last = (int)(p.K - (size_t)(nb - 1) * 128);                    // bytes of the last k-step: 1 ... 128
+    const int last = (int)(K - (size_t)(nb - 1) * 128);                    // bytes of the last k-step: 1 ... 128
 
     // s counts the group's k-steps; chunks that start at or behind K are fetched from the row's first bytes (they are cleared in LDS below)
     auto fetch = [&](int s)
@@ -341,6 +346,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(con
     }
 
     const size_t n = n0 + (size_t)(wn * (TN / WN) + 8 * g);
+    T *Y = reinterpret_cast<T *>(p.Y) + (PARTS ? part * (p.M * p.N) : 0);
 #pragma unroll
     for (int h = 0; h < NN / 2; ++h)
     {
@@ -355,7 +361,7 @@ __global__ __launch_bounds__(64 * WM * WN * GROUPS) void product_tile_kernel(con
             float v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) { v[q] = acc[i][2 * h + q / 4][q % 4] + bias[q]; }
-            if (m < p.M) { store_vals(reinterpret_cast<T *>(p.Y) + m * p.ldy + n + 32 * h, left, v); }
+            if (m < p.M) { store_vals(Y + m * p.ldy + n + 32 * h, left, v); }
         }
     }
 }
@@ -622,6 +628,33 @@ __global__ __launch_bounds__(256) void product_stream_kernel(const ProductParams
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");                       // the loads behind the last tile, before its LDS is another's
 }
 
+// ---- a long k and few values: the parts' sums ----
+// Y = the sum of the parts, in their order, + bias: four values a thread
+template <typename T>
+__global__ __launch_bounds__(256) void product_sum_kernel(const ProductParams p, unsigned parts, unsigned nv)
+{
+    const unsigned e = blockIdx.x * 256 + threadIdx.x, m = e / nv, n = (e - m * nv) * 4;
+    if (m >= p.M) { return; }
+    const int left = (int)min(p.N - n, (size_t)4);
+    const float *w = p.work + m * p.N + n;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (unsigned i0 = 0; i0 < parts; i0 += 8)                               // eight parts' values on their way at a time
+    {
+        float v[8][4];
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i) { load_vals<float>(w + min(i0 + i, parts - 1) * (p.M * p.N), left, v[i]); }
+#pragma unroll
+        for (unsigned i = 0; i < 8; ++i)
+        {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { s[q] += i0 + i < parts ? v[i][q] : 0.0f; }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { s[q] += p.bias && q < left ? p.bias[n + q] : 0.0f; }
+    store_vals(reinterpret_cast<T *>(p.Y) + m * p.ldy + n, left, s);
+}
+
 template <typename T, bool TAIL>
 hipError_t stream_go(const ProductParams &p, hipStream_t s)
 {
@@ -637,11 +670,11 @@ template <typename T, int TM, int TN, int WM, int WN, int STAGES, int GROUPS = 1
 hipError_t tile_go(const ProductParams &p, hipStream_t s)
 {
     constexpr int LDS = GROUPS * (STAGES * (TM + TN) * 128 + 2 * (TM + TN) * 4);
-    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<T, TM, TN, WM, WN, STAGES, GROUPS>);
+    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<T, TM, TN, WM, WN, STAGES, GROUPS, false>);
     const hipError_t e = opt_in_lds_once(k, LDS);
     if (e != hipSuccess) { return e; }
     const unsigned tm = (unsigned)((p.M + TM - 1) / TM), tn = (unsigned)((p.N + TN - 1) / TN);
-    hipLaunchKernelGGL((product_tile_kernel<T, TM, TN, WM, WN, STAGES, GROUPS>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN * GROUPS), LDS, s, p, tm, tn);
+    hipLaunchKernelGGL((product_tile_kernel<T, TM, TN, WM, WN, STAGES, GROUPS, false>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN * GROUPS), LDS, s, p, tm, tn, 1u);
     return hipSuccess;
 }
 
@@ -654,6 +687,34 @@ hipError_t split_go(const ProductParams &p, hipStream_t s)
 }
 
 size_t tiles(const ProductParams &p, size_t tm, size_t tn) { return ((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn); }
+
+// Into how many parts of how many columns the k-steps are split where there is room for their sums: as many as give the CUs two
+// workgroups of 128 x 128 each.  The sums cost a second launch and 8 bytes of traffic for each part's value, 10 us and more.  Measured, whole
+// and in parts, us: 512 x 720 x 31936 69 / 28, 40 x 257 x 100000 181 / 24, 2048 x 2048 x 31936 199 / 151, 512 x 512 x 8192 19.1 / 16.6,
+// but 1024 x 1024 x 8192 20 / 26 and 512 x 512 x 4096 10.5 / 13.9.
+unsigned product_parts(size_t M, size_t N, size_t K, size_t *part)
+{
+    const size_t t = ((M + 127) / 128) * ((N + 127) / 128);
+    if (M <= 16 || t > 256 || K < (t <= 16 ? 8192u : 16384u)) { return 1; }
+    const size_t want = min(512 / t, K / 1024);
+    *part = (K + want * 512 - 1) / (want * 512) * 512;
+    return (unsigned)((K + *part - 1) / *part);
+}
+
+template <typename T>
+hipError_t parts_go(const ProductParams &p, unsigned parts, size_t part, hipStream_t s)
+{
+    constexpr int LDS = 2 * 256 * 128 + 2 * 256 * 4;
+    const void *k = reinterpret_cast<const void *>(&product_tile_kernel<float, 128, 128, 2, 2, 2, 1, true>);
+    const hipError_t e = opt_in_lds_once(k, LDS);
+    if (e != hipSuccess) { return e; }
+    ProductParams q = p;
+    q.part = part; q.bias = nullptr; q.Y = p.work; q.ldy = p.N;
+    const unsigned tm = (unsigned)((p.M + 127) / 128), tn = (unsigned)((p.N + 127) / 128), nv = (unsigned)((p.N + 3) / 4);
+    hipLaunchKernelGGL((product_tile_kernel<float, 128, 128, 2, 2, 2, 1, true>), dim3((tm * tn * parts + 7) / 8 * 8), dim3(256), LDS, s, q, tm, tn, parts);
+    hipLaunchKernelGGL(product_sum_kernel<T>, dim3((unsigned)((p.M * nv + 255) / 256)), dim3(256), 0, s, p, parts, nv);
+    return hipSuccess;
+}
 
 // Which kernel: the largest tile whose last round over the 256 CUs is not mostly empty, since a value then costs the fewest operand bytes.
 // A CU holds one workgroup of 256 x 256, two of 128 x 128 or 128 x 64, three of 64 x 64.  Measured, us:
@@ -680,6 +741,9 @@ hipError_t product_go(const ProductParams &p, hipStream_t s)
     const bool near = p.K > 0 && p.lda < ((size_t)1 << 23) && p.ldb < ((size_t)1 << 23) && p.ldsa < ((size_t)1 << 23) && p.ldsb < ((size_t)1 << 23);
     const size_t t256 = tiles(p, 256, 256), rounds = (t256 + 255) / 256, t64 = tiles(p, 64, 64);
     const bool full = 5 * t256 >= 4 * 256 * rounds, amortized = p.K > 512 || (p.K > 384 && rounds > 1);
+    size_t part = 0;
+    const unsigned parts = product_parts(p.M, p.N, p.K, &part);
+    if (near && parts > 1 && p.work_bytes >= parts * p.M * p.N * sizeof(float)) { return parts_go<T>(p, parts, part, s); }
     if (near && p.M >= 256 && p.N >= 256 && full && amortized) { return p.K % 128 ? stream_go<T, true>(p, s) : stream_go<T, false>(p, s); }
     if (near && tiles(p, 128, 64) > 512) { return tile_go<T, 128, 128, 2, 2, 2>(p, s); }
     if (near && (t64 > 768 || (t64 > 256 && p.K > 4096))) { return tile_go<T, 128, 64, 2, 2, 3>(p, s); }
@@ -689,6 +753,13 @@ hipError_t product_go(const ProductParams &p, hipStream_t s)
 }
 
 }  // namespace
+
+size_t rows_product_work(size_t M, size_t N, size_t K)
+{
+    size_t part = 0;
+    const unsigned parts = product_parts(M, N, K, &part);
+    return parts > 1 ? parts * M * N * sizeof(float) : 0;
+}
 
 hipError_t launch_rows_product(int dtype, const ProductParams &p, hipStream_t s)
 {

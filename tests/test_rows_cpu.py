@@ -46,8 +46,8 @@ def test_empty_calls_succeed_without_a_device():
     assert lib.speech_rows_rms_norm_backward(0, C.byref(_lib.SpeechNormGrad(cols=4, dH=P)), None) == 0
     assert lib.speech_rows_quantize(0, 0, 0, 8, None, 8, None, 16, None, 4, 0, None) == 0
     assert lib.speech_rows_quantize(0, 0, 8, 0, None, 8, None, 16, None, 4, 1, None) == 0
-    assert lib.speech_rows_product(0, 3, 0, 8, 8, None, 16, None, 4, None, 16, None, 4, None, None, 8, None) == 0
-    assert lib.speech_rows_product(0, 3, 8, 0, 8, None, 16, None, 4, None, 16, None, 4, None, None, 8, None) == 0
+    assert lib.speech_rows_product(0, 3, 0, 8, 8, None, 16, None, 4, None, 16, None, 4, None, None, 8, None, 0, None) == 0
+    assert lib.speech_rows_product(0, 3, 8, 0, 8, None, 16, None, 4, None, 16, None, 4, None, None, 8, None, 0, None) == 0
 
 
 @pytest.mark.parametrize("kw,msg", [
@@ -125,6 +125,17 @@ def test_work_sizes(capfd):
     capfd.readouterr()
 
 
+def test_product_work_sizes(capfd):
+    assert api.product_work(2048, 1024, 4096) == 0 and api.product_work(1, 512, 1 << 20) == 0 and api.product_work(8192, 8192, 1 << 16) == 0
+    assert api.product_work(0, 10, 1 << 20) == 0
+    n = api.product_work(512, 720, 31936)
+    assert n > 0 and n % (512 * 720 * 4) == 0 and n // (512 * 720 * 4) <= 31
+    assert _lib.load().speech_rows_product_work(1, 1, 1, None) == 1
+    with pytest.raises(api.SpeechError):
+        api.product_work(1, 1, 1 << 31)
+    capfd.readouterr()
+
+
 @pytest.mark.parametrize("kw,msg", [
     (dict(dtype=1), "unknown dtype 1"),
     (dict(X=None), "null device pointer X"),
@@ -156,11 +167,13 @@ def test_quantize_refuses(kw, msg, capfd):
     (dict(bias=P + 2), "bias is not aligned"),
     (dict(k=1 << 31), "at most 2^30"),
     (dict(rows=1 << 30, cols=1 << 30, ldy=1 << 30), "matrix too large"),
+    (dict(work=P + 8), "work must start on 16 bytes"),
 ])
 def test_product_refuses(kw, msg, capfd):
-    a = dict(dtype=2, rows=10, cols=20, k=30, A=P, lda=32, SA=P + 4096, ldsa=4, B=P + 8192, ldb=32, SB=P + 16384, ldsb=4, bias=None, Y=P + 32768, ldy=20)
+    a = dict(dtype=2, rows=10, cols=20, k=30, A=P, lda=32, SA=P + 4096, ldsa=4, B=P + 8192, ldb=32, SB=P + 16384, ldsb=4, bias=None, Y=P + 32768, ldy=20,
+             work=None, work_bytes=0)
     a.update(kw)
-    args = [a[n] for n in "dtype rows cols k A lda SA ldsa B ldb SB ldsb bias Y ldy".split()]
+    args = [a[n] for n in "dtype rows cols k A lda SA ldsa B ldb SB ldsb bias Y ldy work work_bytes".split()]
     assert _lib.load().speech_rows_product(0, *args, None) == 1
     assert "error in speech_rows_product: " in capfd.readouterr().err and msg in _lib.last_error(), _lib.last_error()
 
@@ -181,6 +194,7 @@ def test_python_refuses_host_tensors_and_types():
         api.quantize(x.int(), x, x)
     q, s = api.held(5, 200, device="cpu")
     assert q.shape == (5, 200) and q.stride(0) == 208 and s.shape == (5, 2) and s.stride(0) == 4
+    assert api.held(5, 720, device="cpu")[0].stride(0) == 768
 
 
 def test_statement_of_the_mask():

@@ -435,6 +435,28 @@ PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 512, 2048), (2, 100, 130), (5, 33, 400)
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("rows,cols,k", PRODUCTS)
 def test_product(rows, cols, k, dt):
+    _product(rows, cols, k, dt)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,k", [(17, 1, 8192), (40, 257, 20000), (130, 140, 9001), (257, 512, 8192), (100, 1999, 8200), (520, 700, 17000), (2000, 1990, 16400)])
+def test_product_in_parts(rows, cols, k, dt):
+    torch = _t()
+    from speech_amd import api
+    need = api.product_work(rows, cols, k)
+    assert need > 0
+    work = torch.full((need + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    qa, sa, qb, sb, z = _product(rows, cols, k, dt, work[:need])
+    assert bool((work[need:] == 0xA5).all()) and not bool((work[:need] == 0xA5).all())
+    whole, short = torch.empty_like(z), torch.empty_like(z)
+    before = work.clone()
+    api.product(qa, sa, qb, sb, whole)
+    api.product(qa, sa, qb, sb, short, work=work[:need - 16])                  # too little: computed whole, nothing left in it
+    torch.cuda.synchronize()
+    assert torch.equal(whole, short) and torch.equal(work, before)
+
+
+def _product(rows, cols, k, dt, work=None):
     torch = _t()
     from speech_amd import api
     rng = np.random.default_rng(15 + k)
@@ -457,16 +479,18 @@ def test_product(rows, cols, k, dt):
     (qa, sa, va), (qb, sb, vb) = put(a), put(b)
     y = Canvas(rows, cols, _type(dt), pad=3, lead=1)
     z = torch.empty(rows, cols, dtype=_type(dt), device="cuda")
-    api.product(qa, sa, qb, sb, y.m, bias=torch.from_numpy(bias).cuda())
-    api.product(qa, sa, qb, sb, z)
+    api.product(qa, sa, qb, sb, y.m, bias=torch.from_numpy(bias).cuda(), work=work)
+    api.product(qa, sa, qb, sb, z, work=work)
     torch.cuda.synchronize()
     unit = _unit(va, vb)
     for got, add in ((_np(y.m), bias.astype(np.float64)), (_np(z), 0.0)):
         want = va @ vb.T + add
-        # 128 products inside the matrix unit, then one addition for each k-step, for each partial sum of at most 64, and the bias
+        # 128 products inside the matrix unit, then one addition for each k-step, for each partial sum (of waves at most 16, of parts one for
+        # eight k-steps: never more than 64 and the k-steps that they save), and the bias
         err = (128 + -(-k // 128) + 64 + 1) * F * (np.abs(va) @ np.abs(vb).T + np.abs(add)) + unit
         _near(got, want, err + U[dt] * (np.abs(want) + err) + TINY[dt] * U[dt], "product")
     assert y.untouched()
+    return qa, sa, qb, sb, z
 
 
 def test_product_places_every_element():
