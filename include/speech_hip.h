@@ -277,7 +277,7 @@ int speech_rows_rms_norm_backward(int device, const speech_norm_grad *args, void
 int speech_rows_rms_norm_work(size_t rows, size_t cols, size_t *bytes);
 
 /* 8-bit form of a matrix: Q holds e4m3 values (4 exponent bits, 3 mantissa bits, largest 448, no infinities), S one byte e for each
-   block of 128 columns of a row, and element (i, j) stands for Q[i][j] 2^(S[i][j / 128] - 127).  A block's scale is the smallest
+   block of 128 columns of a row, and element (i, j) stands for Q[i][j] 2^(S[i][j / 128] - 127), for NaN where S is 255.  A block's scale is the smallest
    power of two (2^-127 at least) that brings its largest finite value to at most 448: a power of two costs a float format no
    precision, is exact to divide by, and is what the matrix units apply by themselves.  Values are rounded to nearest, ties
    to even; NaN and infinities become e4m3 NaN and leave their block's scale alone.

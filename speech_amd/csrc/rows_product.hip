@@ -764,12 +764,16 @@ size_t rows_product_work(size_t M, size_t N, size_t K)
 hipError_t launch_rows_product(int dtype, const ProductParams &p, hipStream_t s)
 {
     hipError_t e = hipErrorInvalidValue;
-    switch (dtype)
+    try                                                                      // a kernel's first call notes it in a table on the heap
     {
-        case SPEECH_BF16: e = product_go<__bf16>(p, s); break;
-        case SPEECH_F16: e = product_go<_Float16>(p, s); break;
-        default: break;
+        switch (dtype)
+        {
+            case SPEECH_BF16: e = product_go<__bf16>(p, s); break;
+            case SPEECH_F16: e = product_go<_Float16>(p, s); break;
+            default: break;
+        }
     }
+    catch (...) { e = hipErrorOutOfMemory; }
     return e != hipSuccess ? e : hipGetLastError();
 }
 

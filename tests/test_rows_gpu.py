@@ -533,6 +533,111 @@ def test_product_keeps_nan_in_its_row_and_column():
         assert np.array_equal(_np(y), want, equal_nan=True)
 
 
+@pytest.mark.parametrize("rows,cols,k", [(20, 40, 300), (600, 700, 300), (1000, 1030, 640), (4096, 4096, 640), (40, 200, 8200)])
+def test_product_of_extreme_scales(rows, cols, k):
+    """255 is NaN for its rows and columns only; the largest and the smallest scales meet in a finite product"""
+    torch = _t()
+    from speech_amd import api
+    qa, sa = api.held(rows, k)
+    qb, sb = api.held(cols, k)
+    qa.copy_(torch.ones(rows, k, device="cuda"))
+    qb.copy_(torch.ones(cols, k, device="cuda"))
+    sa.fill_(127)
+    sb.fill_(127)
+    sa[5, 1], sb[7, 0] = 255, 255
+    sa[3], sb[9] = 254, 0                                                      # 2^127 and 2^-127
+    y = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    need = api.product_work(rows, cols, k)
+    api.product(qa, sa, qb, sb, y, work=torch.empty(need, dtype=torch.uint8, device="cuda") if need else None)
+    torch.cuda.synchronize()
+    bad = torch.isnan(y)
+    assert bool(bad[5].all()) and bool(bad[:, 7].all()) and int(bad.sum()) == rows + cols - 1
+    one = torch.tensor(float(k)).bfloat16().item()
+    assert y[3, 9].item() == one and y[0, 0].item() == one and y[rows - 1, cols - 1].item() == one
+    assert torch.isinf(y[3, 0]).item() and y[0, 9].item() == torch.tensor(k * 2.0 ** -127).bfloat16().item()
+
+
+def test_long_offsets():
+    """matrices of more than 2^31 elements: the last rows and columns, bit for bit what the same calls on them alone give"""
+    torch = _t()
+    from speech_amd import api
+    rows, cols, n, last = 2200000, 1024, 256, 300
+    X = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(3))
+    w = torch.linspace(0.5, 1.5, cols, device="cuda")
+    q, s = api.held(rows, cols)
+    rstd = torch.empty(rows, device="cuda")
+    api.rms_norm(X, w, Q=q, S=s, rstd=rstd)
+    tail = X[-last:].clone()
+    qt, st = api.held(last, cols)
+    rt = torch.empty(last, device="cuda")
+    api.rms_norm(tail, w, Q=qt, S=st, rstd=rt)
+    torch.cuda.synchronize()
+    eq = lambda a, b: torch.equal(a.view(torch.uint8), b.view(torch.uint8))  # noqa: E731
+    assert eq(q[-last:], qt) and eq(s[-last:], st) and torch.equal(rstd[-last:], rt)
+    api.quantize(X, q, s)
+    api.quantize(tail, qt, st)
+    torch.cuda.synchronize()
+    assert eq(q[-last:], qt) and eq(s[-last:], st)
+
+    qb, sb = api.held(n, cols)
+    api.quantize(X[:n], qb, sb)
+    y = torch.empty(rows, n, device="cuda", dtype=torch.bfloat16)
+    api.product(q, s, qb, sb, y)
+    torch.cuda.synchronize()
+    va, vb = (R.stands_for(a.view(torch.uint8).cpu().numpy(), b.cpu().numpy()) for a, b in ((qt, st), (qb, sb)))
+    want = va @ vb.T
+    err = (128 + 8 + 64) * F * (np.abs(va) @ np.abs(vb).T) + _unit(va, vb)
+    _near(_np(y[-last:]), want, err + U["bf16"] * (np.abs(want) + err), "last rows")
+    del y, q, s
+
+    work = torch.empty(api.rms_norm_work(rows, cols), dtype=torch.uint8, device="cuda")
+    dH, dt = torch.empty_like(X), torch.empty_like(tail)
+    api.rms_norm_backward(X, X, w, rstd, dH, dW=torch.empty(cols, device="cuda"), work=work)
+    api.rms_norm_backward(tail, tail, w, rt, dt)
+    torch.cuda.synchronize()
+    assert torch.equal(dH[-last:], dt)
+    del dH
+
+    q, s = api.held(cols, rows)
+    api.quantize(X, q, s, transpose=True)
+    part = X[:, -64:].contiguous()
+    qt, st = api.held(64, rows)
+    api.quantize(part, qt, st, transpose=True)
+    torch.cuda.synchronize()
+    assert eq(q[-64:], qt) and eq(s[-64:], st)
+
+
+def test_product_in_parts_in_replayed_graphs():
+    """two graphs with a work array each, replayed in turn with eager calls between"""
+    torch = _t()
+    from speech_amd import api
+    rows, cols, k = 96, 200, 8200
+    gen = torch.Generator("cuda").manual_seed(4)
+    X = [torch.empty(r, k, device="cuda").normal_(generator=gen) for r in (rows, cols)]
+    (qa, sa), (qb, sb) = api.held(rows, k), api.held(cols, k)
+    work = [torch.empty(api.product_work(rows, cols, k), dtype=torch.uint8, device="cuda") for _ in range(3)]
+    out = [torch.zeros(rows, cols, device="cuda", dtype=torch.float16) for _ in range(3)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            st = torch.cuda.current_stream().cuda_stream
+            if i == 0:
+                api.quantize(X[0], qa, sa, stream=st)
+                api.quantize(X[1], qb, sb, stream=st)
+            api.product(qa, sa, qb, sb, out[i], work=work[i], stream=st)
+    for _ in range(4):
+        X[0].normal_(generator=gen)
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        api.product(qa, sa, qb, sb, out[2], work=work[2])
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[2]) and bool(out[2].any())
+        for o in out:
+            o.zero_()
+
+
 def test_product_gradients_against_the_formula():
     """dX = q(dY) q(W^T)^T and dW = q(dY^T) q(X^T)^T: within the 8-bit rounding (2^-4 of each factor; below a block's
     normal range 2^-10 of its scale, that is 2^-18 of the block's largest value) of dY W and dY^T X, and the result's own"""
