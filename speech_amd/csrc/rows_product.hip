@@ -69,7 +69,8 @@ __device__ __forceinline__ v8i load_frag(const uint8_t *row, size_t k, size_t K)
 
 // Few values, any K: a workgroup computes 16 MT x 16 NN of them, its WAVES waves split the k-steps, and their sums are added in wave order
 // through LDS.  Operands come straight from memory: nothing is read twice that another workgroup's read would not have left in
-// L2.  With one row of A this is the reading of the weights.
+// L2.  With one row of A this is the reading of the weights, bound by that: 1 x 4096 x 4096 in 4.6 us, 8 x 8192 x 8192 in 14.8 (4.5 TB/s);
+// 1 x 1024 x 1024 in 2.7, a launch and three trips to memory.
 template <typename T, int MT, int NN, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void product_split_kernel(const ProductParams p, unsigned ntiles)
 {
