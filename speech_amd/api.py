@@ -477,7 +477,7 @@ def _rows_arg(t, what, device, dtypes, rows, cols, pad=1):
     elif ld < cols or (pad > 1 and ld % pad):
         raise ValueError("%s has a row stride of %d for %d columns%s" % (what, ld, cols, "" if pad == 1 else ": a multiple of %d is needed" % pad))
     p = t.data_ptr()
-    if pad > 1 and rows and cols and (t.storage_offset() + (rows - 1) * ld + full > t.untyped_storage().nbytes() or p % pad):
+    if pad > 1 and rows and cols and (p % pad or (full > cols and t.storage_offset() + (rows - 1) * ld + full > t.untyped_storage().nbytes())):
         raise ValueError("%s needs rows that start on %d bytes and have memory up to the next %d (see held)" % (what, pad, pad))
     return p, ld
 
