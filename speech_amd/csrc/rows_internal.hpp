@@ -83,6 +83,39 @@ __device__ __forceinline__ void load_vals(const T *p, int n, F (&v)[N])
     }
 }
 
+// the first `left` < 16 bytes of four words, in at most one store for each power of two
+template <typename T>
+__device__ __forceinline__ void store_bytes(T *p, int left, unsigned a, unsigned b, unsigned c, unsigned d)
+{
+    uint8_t *q = reinterpret_cast<uint8_t *>(p);
+    if (left & 8)
+    {
+        typename VecOf<T, 8 / sizeof(T)>::type x;
+        const uint2 w = make_uint2(a, b);
+        __builtin_memcpy(&x, &w, 8);
+        *reinterpret_cast<typename VecOf<T, 8 / sizeof(T)>::type *>(q) = x;
+        q += 8; a = c; b = d;
+    }
+    if constexpr (sizeof(T) <= 4)
+    {
+        if (left & 4)
+        {
+            typename VecOf<T, 4 / sizeof(T)>::type x;
+            __builtin_memcpy(&x, &a, 4);
+            *reinterpret_cast<typename VecOf<T, 4 / sizeof(T)>::type *>(q) = x;
+            q += 4; a = b;
+        }
+    }
+    if constexpr (sizeof(T) <= 2)
+    {
+        if (left & 2)
+        {
+            const uint16_t h = (uint16_t)a;
+            __builtin_memcpy(q, &h, 2);
+        }
+    }
+}
+
 template <typename F, typename T, int N>
 __device__ __forceinline__ void store_vals(T *p, int n, const F (&v)[N])
 {
@@ -93,10 +126,49 @@ __device__ __forceinline__ void store_vals(T *p, int n, const F (&v)[N])
         for (int i = 0; i < N; ++i) { x[i] = (T)v[i]; }
         *reinterpret_cast<typename VecOf<T, N>::type *>(p) = x;
     }
+    else if constexpr (N * sizeof(T) == 16)
+    {
+        typename VecOf<T, N>::type x;
+#pragma unroll
+        for (int i = 0; i < N; ++i) { x[i] = (T)v[i]; }
+        uint4 w;
+        __builtin_memcpy(&w, &x, 16);
+        if (n > 0) { store_bytes(p, n * (int)sizeof(T), w.x, w.y, w.z, w.w); }
+    }
     else
     {
 #pragma unroll
         for (int i = 0; i < N; ++i) { if (i < n) { p[i] = (T)v[i]; } }
+    }
+}
+
+// A row's vectors, all loaded before the first is looked at.  The last one of a row whose columns are no whole vectors is read whole where
+// memory follows (a row that has another behind it has some for any vector that starts inside it) and its rest set to 0 in row_vals:
+// element by element it would cost up to seven loads more, and twice the time of the whole pass (42184 x 455).  Lanes behind the row hold 0.
+template <typename T> using RowVec = typename VecOf<T, vec_of<T>()>::type;
+template <typename T> __device__ __forceinline__ bool row_has_more(size_t row, size_t rows, size_t ld) { return row + 1 < rows && ld >= (size_t)vec_of<T>(); }
+template <typename T>
+__device__ __forceinline__ RowVec<T> row_vec(const T *p, int n, bool more)
+{
+    constexpr int N = vec_of<T>();
+    RowVec<T> x;
+    if (n >= N || (more && n > 0)) { x = *reinterpret_cast<const RowVec<T> *>(p); }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { x[i] = i < n ? p[i] : (T)0; }
+    }
+    return x;
+}
+template <typename T, typename F, int N>
+__device__ __forceinline__ void row_vals(const RowVec<T> &x, int n, bool ragged, F (&v)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) { v[i] = (F)x[i]; }
+    if (ragged)
+    {
+#pragma unroll
+        for (int i = 1; i < N; ++i) { v[i] = i < n ? v[i] : (F)0; }
     }
 }
 

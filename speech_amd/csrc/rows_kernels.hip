@@ -64,12 +64,13 @@ __global__ __launch_bounds__(NT) void dropout_kernel(const T *X, T *Y, size_t ld
     const size_t first = (size_t)blockIdx.x * NT + threadIdx.x;
     size_t row = first / (unsigned)nv;
     int v = (int)(first - row * (unsigned)nv);
+    const bool ragged = cols % N != 0;
     const F scale = (F)d.scale;
     while (row < rows)
     {
         const int c = v * N;
         F x[N];
-        load_vals<F>(X + row * ldx + c, cols - c, x);
+        row_vals<T>(row_vec(X + row * ldx + c, cols - c, row_has_more<T>(row, rows, ldx)), cols - c, ragged, x);
         if (d.on)
         {
             const unsigned long long fk = drop_row_key(ku, d, row);
@@ -154,25 +155,19 @@ __device__ __forceinline__ void norm_input(const NormParams &p, size_t row, int 
 
 // The same for CH vectors of a row, all loads before the first use; 0 behind the row's end.
 template <typename T, int TPR, int CH, int N>
-__device__ __forceinline__ void norm_inputs(const NormParams &p, size_t row, int t, unsigned long long fk, float (&h)[CH][N])
+__device__ __forceinline__ void norm_inputs(const NormParams &p, size_t row, int t, unsigned long long fk, bool ragged, float (&h)[CH][N])
 {
     const T *X = reinterpret_cast<const T *>(p.X) + row * p.ldx, *R = reinterpret_cast<const T *>(p.R) + row * p.ldr;
-    float r[CH][N];
+    RowVec<T> x[CH], r[CH];
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
-    {
-        const int c = (k * TPR + t) * N;
-        load_vals<float>(X + c, p.cols - c, h[k]);
-    }
+    for (int k = 0; k < CH; ++k) { const int c = (k * TPR + t) * N; x[k] = row_vec(X + c, p.cols - c, row_has_more<T>(row, p.rows, p.ldx)); }
     if (p.R)
     {
 #pragma unroll
-        for (int k = 0; k < CH; ++k)
-        {
-            const int c = (k * TPR + t) * N;
-            load_vals<float>(R + c, p.cols - c, r[k]);
-        }
+        for (int k = 0; k < CH; ++k) { const int c = (k * TPR + t) * N; r[k] = row_vec(R + c, p.cols - c, row_has_more<T>(row, p.rows, p.ldr)); }
     }
+#pragma unroll
+    for (int k = 0; k < CH; ++k) { row_vals<T>(x[k], p.cols - (k * TPR + t) * N, ragged, h[k]); }
     if (p.drop.on)
     {
         const float scale = (float)p.drop.scale;
@@ -188,8 +183,10 @@ __device__ __forceinline__ void norm_inputs(const NormParams &p, size_t row, int
 #pragma unroll
         for (int k = 0; k < CH; ++k)
         {
+            float v[N];
+            row_vals<T>(r[k], p.cols - (k * TPR + t) * N, ragged, v);
 #pragma unroll
-            for (int i = 0; i < N; ++i) { h[k][i] += r[k][i]; }
+            for (int i = 0; i < N; ++i) { h[k][i] += v[i]; }
         }
     }
 #pragma unroll
@@ -213,10 +210,12 @@ __device__ __forceinline__ void store_e4m3(uint8_t *q, int n, const float (&y)[N
         if (N == 8) { *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[N / 4 - 1]); }
         else { *reinterpret_cast<unsigned *>(q) = w[0]; }
     }
-    else
+    else if (n > 0)                                                          // four, two and one byte of what is left
     {
-#pragma unroll
-        for (int i = 0; i < N; ++i) { if (i < n) { q[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4))); } }
+        unsigned a = w[0];
+        if (N == 8 && n & 4) { *reinterpret_cast<unsigned *>(q) = a; q += 4; a = w[N / 4 - 1]; }
+        if (n & 2) { *reinterpret_cast<uint16_t *>(q) = (uint16_t)a; q += 2; a >>= 16; }
+        if (n & 1) { *q = (uint8_t)a; }
     }
 }
 
@@ -224,14 +223,15 @@ __device__ __forceinline__ void store_e4m3(uint8_t *q, int n, const float (&y)[N
 // there for all of a thread's rows.  Bound by HBM: 31936 x 1024 bf16 with residual and dropout, 262 MB, in 55 us (4.8 TB/s); 7984 x 1024
 // to 8 bits, 57 MB, in 12.4 us (4.6 TB/s); one row of 2048 in 2.7 us, a launch and two trips to memory.
 template <typename T, int TPR, int CH>
-__global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormParams p)
+__global__ __launch_bounds__(TPR > 64 ? TPR : NT) void norm_kernel(const NormParams p)
 {
-    constexpr int N = vec_of<T>(), NTH = TPR > NT ? TPR : NT, RPW = NTH / TPR, LB = ROWS_BLOCK / N;
+    constexpr int N = vec_of<T>(), NTH = TPR > 64 ? TPR : NT, RPW = NTH / TPR, LB = ROWS_BLOCK / N;
     __shared__ float sh[2 * (NTH / 64)];
     const int t = threadIdx.x % TPR;
     int flip = 0;
     const unsigned long long ku = drop_layer_key(p.drop);
     const int nb = (p.cols + ROWS_BLOCK - 1) / ROWS_BLOCK;
+    const bool ragged = p.cols % N != 0;
     constexpr bool HOLD = TPR < 1024;                                        // 1024 threads have 128 registers each
     float w[CH][N];
     if (HOLD)
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT) void norm_kernel(const NormPar
     {
         const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
         float h[CH][N];
-        norm_inputs<T, TPR>(p, row, t, fk, h);
+        norm_inputs<T, TPR>(p, row, t, fk, ragged, h);
         float ss = 0.0f;
 #pragma unroll
         for (int k = 0; k < CH; ++k)
@@ -388,12 +388,13 @@ __device__ __forceinline__ void grad_store(const NormGradParams &p, size_t row, 
 // Registers for four waves a SIMD up to 16 values a thread, two above: the grid is sized for that.
 // Bound by HBM: 31936 x 1024 bf16 with residual and dropout, 327 MB, in 71 us (4.6 TB/s), and 5 us for the partial sums.
 template <typename T, int TPR, int CH>
-__global__ __launch_bounds__(TPR > NT ? TPR : NT, TPR > NT ? 4 : CH * vec_of<T>() <= 16 ? 4 : 2) void norm_grad_kernel(const NormGradParams p)
+__global__ __launch_bounds__(TPR > 64 ? TPR : NT, TPR > NT ? 4 : CH * vec_of<T>() <= 16 ? 4 : 2) void norm_grad_kernel(const NormGradParams p)
 {
-    constexpr int N = vec_of<T>(), NTH = TPR > NT ? TPR : NT, RPW = NTH / TPR;
+    constexpr int N = vec_of<T>(), NTH = TPR > 64 ? TPR : NT, RPW = NTH / TPR;
     __shared__ float sh[2 * (NTH / 64)];
     __shared__ float part[RPW > 1 ? NTH * N : 1];
     const int t = threadIdx.x % TPR;
+    const bool ragged = p.cols % N != 0;
     int flip = 0;
     const unsigned long long ku = drop_layer_key(p.drop);
     float acc[CH][N];
@@ -407,14 +408,29 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT, TPR > NT ? 4 : CH * vec_of<T>(
     {
         const unsigned long long fk = p.drop.on ? drop_row_key(ku, p.drop, row) : 0ull;
         const float rstd = p.rstd[row];
-        float g[CH][N], h[CH][N], r[CH][N];
+        RowVec<T> xg[CH], xh[CH], xr[CH];
 #pragma unroll
         for (int k = 0; k < CH; ++k)
         {
             const int c = (k * TPR + t) * N;
-            load_vals<float>(reinterpret_cast<const T *>(p.dY) + row * p.lddy + c, p.cols - c, g[k]);
-            load_vals<float>(reinterpret_cast<const T *>(p.H) + row * p.ldh + c, p.cols - c, h[k]);
-            if (p.dR) { load_vals<float>(reinterpret_cast<const T *>(p.dR) + row * p.lddr + c, p.cols - c, r[k]); }
+            xg[k] = row_vec(reinterpret_cast<const T *>(p.dY) + row * p.lddy + c, p.cols - c, row_has_more<T>(row, p.rows, p.lddy));
+            xh[k] = row_vec(reinterpret_cast<const T *>(p.H) + row * p.ldh + c, p.cols - c, row_has_more<T>(row, p.rows, p.ldh));
+        }
+        if (p.dR)
+        {
+#pragma unroll
+            for (int k = 0; k < CH; ++k)
+            {
+                const int c = (k * TPR + t) * N;
+                xr[k] = row_vec(reinterpret_cast<const T *>(p.dR) + row * p.lddr + c, p.cols - c, row_has_more<T>(row, p.rows, p.lddr));
+            }
+        }
+        float g[CH][N], h[CH][N];
+#pragma unroll
+        for (int k = 0; k < CH; ++k)
+        {
+            row_vals<T>(xg[k], p.cols - (k * TPR + t) * N, ragged, g[k]);
+            row_vals<T>(xh[k], p.cols - (k * TPR + t) * N, ragged, h[k]);
         }
         float s = 0.0f;
 #pragma unroll
@@ -437,7 +453,14 @@ __global__ __launch_bounds__(TPR > NT ? TPR : NT, TPR > NT ? 4 : CH * vec_of<T>(
         {
             const int c = (k * TPR + t) * N;
 #pragma unroll
-            for (int i = 0; i < N; ++i) { g[k][i] = g[k][i] * rstd - h[k][i] * coef + (p.dR ? r[k][i] : 0.0f); }
+            for (int i = 0; i < N; ++i) { g[k][i] = g[k][i] * rstd - h[k][i] * coef; }
+            if (p.dR)
+            {
+                float r[N];
+                row_vals<T>(xr[k], p.cols - c, ragged, r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) { g[k][i] += r[i]; }
+            }
             grad_store<T>(p, row, c, fk, g[k]);
         }
     }
@@ -573,6 +596,7 @@ __global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, si
                                                       size_t step_row, int step_b)
 {
     constexpr int V = vec_of<T>();
+    const bool ragged = cols % V != 0;
     const int l = threadIdx.x & 15;
     const size_t first = (size_t)blockIdx.x * (NT / 16) + threadIdx.x / 16;
     size_t row = first / (unsigned)nb;
@@ -581,7 +605,7 @@ __global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, si
     {
         size_t rr[2];
         int cc[2];
-        float x[2][8];
+        RowVec<T> raw[2][8 / V];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
         {
@@ -589,10 +613,7 @@ __global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, si
 #pragma unroll
             for (int k = 0; k < 8; k += V)
             {
-                float v[V];
-                load_vals<float>(X + row * ldx + cc[u] + k, row < rows ? cols - cc[u] - k : 0, v);
-#pragma unroll
-                for (int i = 0; i < V; ++i) { x[u][k + i] = v[i]; }
+                raw[u][k / V] = row_vec(X + row * ldx + cc[u] + k, row < rows ? cols - cc[u] - k : 0, row_has_more<T>(row, rows, ldx));
             }
             row += step_row; b += step_b;
             if (b >= nb) { b -= nb; ++row; }
@@ -600,13 +621,22 @@ __global__ __launch_bounds__(NT) void quantize_kernel(const T *X, size_t ldx, si
 #pragma unroll
         for (int u = 0; u < 2; ++u)
         {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k += V)
+            {
+                float v[V];
+                row_vals<T>(raw[u][k / V], cols - cc[u] - k, ragged, v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) { x[k + i] = v[i]; }
+            }
             unsigned amax = 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) { amax = max(amax, finite_bits(x[u][i])); }
+            for (int i = 0; i < 8; ++i) { amax = max(amax, finite_bits(x[i])); }
             const unsigned e = block_exponent(lanes_max<16>(amax));
             if (rr[u] < rows)
             {
-                store_e4m3(Q + rr[u] * ldq + cc[u], cols - cc[u], x[u], block_factor(e));
+                store_e4m3(Q + rr[u] * ldq + cc[u], cols - cc[u], x, block_factor(e));
                 if (l == 0) { S[rr[u] * lds + cc[u] / ROWS_BLOCK] = (uint8_t)e; }
             }
         }
@@ -667,21 +697,30 @@ __global__ __launch_bounds__(NT) void quantize_transpose_kernel(const T *X, size
 }
 
 // ---- launches ----
-// Threads a row and vectors a thread: a row that fits 16 or 64 lanes needs no barrier, but where there are no more rows than CUs a wave
-// with several vectors a lane would be all that a CU has (1 x 2048 bf16: a wave 6.0 us, four waves 5.0); up to 1024 threads x 4
-// vectors hold a row (16 384 floats, 32 768 16-bit values), beyond that it is walked twice.
-#define ROWS_BY_WIDTH(T, rows, cols, GO, WIDE)                                                               \
+// Threads a row and vectors a thread: the fewest lanes that stay empty, with 16 (32-bit values: 32, a block's 128 columns) or 64 lanes where the
+// row fits, which need no barrier.  31936 ... 60000 rows of 16-bit values, residual and dropout, us: 192 columns 24.7 (64 threads of one vector:
+// 44.9), 257 35.7 (52), 1216 42.5 (64 x 4: 54, 256 x 1: 57), 2048 53.7 (64 x 4: 54.7, 256 x 1: 59.7), 4096 52.9.  The backward pass has
+// at most 1024 workgroups, so it wants more threads in each: 2048 71 (128 x 2: 79).  Where there are no more rows than CUs a wave with several
+// vectors a lane would be all that a CU has (1 x 2048 bf16: a wave 6.0 us, four waves 5.0); up to 1024 threads x 4 vectors hold a row (16 384
+// floats, 32 768 16-bit values), beyond that it is walked twice; so is the backward pass's row of more than 16 384 16-bit values, for which 128
+// registers a thread are too few (2000 x 16384: 1024 x 2 102 us, 1024 x 4 445; 1500 x 33000, walked twice, 196).
+#define ROWS_BY_WIDTH(T, rows, cols, BACK, GO, WIDE)                                                         \
     do {                                                                                                     \
+        constexpr int block_ = ROWS_BLOCK / vec_of<T>();                                                     \
         const int nv_ = ((cols) + vec_of<T>() - 1) / vec_of<T>();                                            \
         if (nv_ <= 16) { GO(16, 1); }                                                                        \
-        else if (sizeof(T) == 4 && nv_ <= 32) { GO(16, 2); }                                                 \
+        else if (nv_ <= 32) { GO(16, 2); }                                                                   \
+        else if (nv_ <= 48) { GO(block_, 48 / block_ + (48 % block_ ? 1 : 0)); }                             \
         else if (nv_ <= 64) { GO(64, 1); }                                                                   \
         else if (nv_ <= 256 && (rows) <= 256) { GO(256, 1); }                                                \
         else if (nv_ <= 128) { GO(64, 2); }                                                                  \
-        else if (nv_ <= 256) { GO(64, 4); }                                                                  \
+        else if (nv_ <= 192) { GO(64, 3); }                                                                  \
+        else if (nv_ <= 256) { GO((BACK ? 256 : 128), (BACK ? 1 : 2)); }                                     \
         else if (nv_ <= 512) { GO(256, 2); }                                                                 \
+        else if (nv_ <= 768) { GO(256, 3); }                                                                 \
         else if (nv_ <= 1024) { GO(256, 4); }                                                                \
-        else if (nv_ <= 4096) { GO(1024, 4); }                                                               \
+        else if (nv_ <= 2048) { GO(1024, 2); }                                                               \
+        else if (nv_ <= 4096 && !(BACK && sizeof(T) == 2)) { if constexpr (!(BACK && sizeof(T) == 2)) { GO(1024, 4); } } \
         else { WIDE; }                                                                                       \
     } while (0)
 
@@ -692,11 +731,11 @@ void norm_go(const NormParams &p, hipStream_t s)
 {
 #define GO(TPR, CH)                                                                                          \
     do {                                                                                                     \
-        constexpr int nth = TPR > NT ? TPR : NT, rpw = nth / TPR;                                            \
+        constexpr int nth = (TPR) > 64 ? (TPR) : NT, rpw = nth / (TPR);                                      \
         const size_t g = (p.rows + rpw - 1) / rpw;                                                           \
-        hipLaunchKernelGGL((norm_kernel<T, TPR, CH>), dim3((unsigned)(g < NORM_MAX_WG ? g : NORM_MAX_WG)), dim3(nth), 0, s, p); \
+        hipLaunchKernelGGL((norm_kernel<T, (TPR), (CH)>), dim3((unsigned)(g < NORM_MAX_WG ? g : NORM_MAX_WG)), dim3(nth), 0, s, p); \
     } while (0)
-    ROWS_BY_WIDTH(T, p.rows, p.cols, GO, hipLaunchKernelGGL(norm_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p));
+    ROWS_BY_WIDTH(T, p.rows, p.cols, false, GO, hipLaunchKernelGGL(norm_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p));
 #undef GO
 }
 
@@ -706,10 +745,10 @@ void norm_grad_go(const NormGradParams &p, hipStream_t s)
     int groups = 0;
 #define GO(TPR, CH)                                                                                          \
     do {                                                                                                     \
-        constexpr int nth = TPR > NT ? TPR : NT, rpw = nth / TPR;                                            \
+        constexpr int nth = (TPR) > 64 ? (TPR) : NT, rpw = nth / (TPR);                                      \
         const size_t g = (p.rows + rpw - 1) / rpw;                                                           \
         groups = (int)(g < ROWS_GRAD_MAX_WG ? g : ROWS_GRAD_MAX_WG);                                         \
-        if (groups) { hipLaunchKernelGGL((norm_grad_kernel<T, TPR, CH>), dim3((unsigned)groups), dim3(nth), 0, s, p); } \
+        if (groups) { hipLaunchKernelGGL((norm_grad_kernel<T, (TPR), (CH)>), dim3((unsigned)groups), dim3(nth), 0, s, p); } \
     } while (0)
 #define WIDE                                                                                                 \
     do {                                                                                                     \
@@ -717,7 +756,7 @@ void norm_grad_go(const NormGradParams &p, hipStream_t s)
         if (p.dW && groups) { hipLaunchKernelGGL(norm_grad_weight_kernel<T>, dim3((unsigned)((p.cols + NT - 1) / NT), (unsigned)groups), dim3(NT), 0, s, p, groups); } \
         if (groups) { hipLaunchKernelGGL(norm_grad_wide_kernel<T>, dim3((unsigned)(p.rows < NORM_MAX_WG ? p.rows : NORM_MAX_WG)), dim3(NT), 0, s, p); } \
     } while (0)
-    ROWS_BY_WIDTH(T, p.rows, p.cols, GO, WIDE);
+    ROWS_BY_WIDTH(T, p.rows, p.cols, true, GO, WIDE);
 #undef WIDE
 #undef GO
     if (p.dW) { hipLaunchKernelGGL(norm_grad_reduce_kernel, dim3((unsigned)((p.cols + 31) / 32)), dim3(1024), 0, s, p.work, p.dW, p.cols, groups); }

@@ -64,7 +64,8 @@ def _near(got, want, bound, what):
     assert np.isfinite(got).all() and (off <= 0).all(), "%s: worst %.3g over at %s" % (what, off.max(), np.unravel_index(np.argmax(off), off.shape))
 
 
-SIZES = [(1, 1), (1, 13), (5, 23), (98, 80), (3, 128), (7, 129), (33, 257), (2, 511), (9, 512), (4, 1000), (5, 1024), (3, 2049), (2, 4097), (3, 8200), (2, 16385), (2, 33000), (1, 40001)]
+SIZES = [(1, 1), (1, 13), (5, 23), (98, 80), (3, 128), (7, 129), (33, 257), (2, 511), (9, 512), (4, 1000), (5, 1024), (3, 2049), (2, 4097), (3, 8200), (2, 16385), (2, 33000), (1, 40001),
+         (1000, 150), (400, 380), (300, 1000), (290, 1219), (270, 1536), (270, 2047), (265, 2305), (260, 4100), (260, 6001), (3, 12000), (2, 20000)]
 
 
 # ---- dropout ----
