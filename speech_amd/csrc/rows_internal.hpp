@@ -83,36 +83,29 @@ __device__ __forceinline__ void load_vals(const T *p, int n, F (&v)[N])
     }
 }
 
-// the first `left` < 16 bytes of four words, in at most one store for each power of two
+// the first n < 8 of eight 16-bit values in four words, in at most three stores
 template <typename T>
-__device__ __forceinline__ void store_bytes(T *p, int left, unsigned a, unsigned b, unsigned c, unsigned d)
+__device__ __forceinline__ void store_part(T *p, int n, unsigned a, unsigned b, unsigned c, unsigned d)
 {
-    uint8_t *q = reinterpret_cast<uint8_t *>(p);
-    if (left & 8)
+    if (n & 4)
     {
-        typename VecOf<T, 8 / sizeof(T)>::type x;
+        typename VecOf<T, 4>::type x;
         const uint2 w = make_uint2(a, b);
         __builtin_memcpy(&x, &w, 8);
-        *reinterpret_cast<typename VecOf<T, 8 / sizeof(T)>::type *>(q) = x;
-        q += 8; a = c; b = d;
+        *reinterpret_cast<typename VecOf<T, 4>::type *>(p) = x;
+        p += 4; a = c; b = d;
     }
-    if constexpr (sizeof(T) <= 4)
+    if (n & 2)
     {
-        if (left & 4)
-        {
-            typename VecOf<T, 4 / sizeof(T)>::type x;
-            __builtin_memcpy(&x, &a, 4);
-            *reinterpret_cast<typename VecOf<T, 4 / sizeof(T)>::type *>(q) = x;
-            q += 4; a = b;
-        }
+        typename VecOf<T, 2>::type x;
+        __builtin_memcpy(&x, &a, 4);
+        *reinterpret_cast<typename VecOf<T, 2>::type *>(p) = x;
+        p += 2; a = b;
     }
-    if constexpr (sizeof(T) <= 2)
+    if (n & 1)
     {
-        if (left & 2)
-        {
-            const uint16_t h = (uint16_t)a;
-            __builtin_memcpy(q, &h, 2);
-        }
+        const uint16_t h = (uint16_t)a;
+        __builtin_memcpy(p, &h, 2);
     }
 }
 
@@ -126,14 +119,14 @@ __device__ __forceinline__ void store_vals(T *p, int n, const F (&v)[N])
         for (int i = 0; i < N; ++i) { x[i] = (T)v[i]; }
         *reinterpret_cast<typename VecOf<T, N>::type *>(p) = x;
     }
-    else if constexpr (N * sizeof(T) == 16)
+    else if constexpr (N == 8 && sizeof(T) == 2)                             // of four floats at most three are left: one by one
     {
         typename VecOf<T, N>::type x;
 #pragma unroll
         for (int i = 0; i < N; ++i) { x[i] = (T)v[i]; }
         uint4 w;
         __builtin_memcpy(&w, &x, 16);
-        if (n > 0) { store_bytes(p, n * (int)sizeof(T), w.x, w.y, w.z, w.w); }
+        if (n > 0) { store_part(p, n, w.x, w.y, w.z, w.w); }
     }
     else
     {

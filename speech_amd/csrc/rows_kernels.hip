@@ -64,13 +64,15 @@ __global__ __launch_bounds__(NT) void dropout_kernel(const T *X, T *Y, size_t ld
     const size_t first = (size_t)blockIdx.x * NT + threadIdx.x;
     size_t row = first / (unsigned)nv;
     int v = (int)(first - row * (unsigned)nv);
-    const bool ragged = cols % N != 0;
     const F scale = (F)d.scale;
     while (row < rows)
     {
         const int c = v * N;
         F x[N];
-        row_vals<T>(row_vec(X + row * ldx + c, cols - c, row_has_more<T>(row, rows, ldx)), cols - c, ragged, x);
+        // 16-bit values: the last vector whole, what is behind the row is not stored (42184 x 455: 21.9 -> 16.5 us); of wider ones at most three are
+        // left over, and one by one they are faster (29940 x 257 f32: 11.2 us, whole 11.7)
+        if constexpr (sizeof(T) == 2) { row_vals<T>(row_vec(X + row * ldx + c, cols - c, row_has_more<T>(row, rows, ldx)), cols - c, false, x); }
+        else { load_vals<F>(X + row * ldx + c, cols - c, x); }
         if (d.on)
         {
             const unsigned long long fk = drop_row_key(ku, d, row);
