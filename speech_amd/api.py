@@ -607,9 +607,20 @@ def product_work(rows, cols, k):
     return n.value
 
 
+def _product_room(rows, cols, k, dev, stream):
+    """room for a product's parts, or None.  The allocator may hand it out again to later work on the current stream, which comes after
+    the product's; on any other stream it would not"""
+    import torch
+    need = product_work(rows, cols, k)
+    if need == 0 or torch.cuda.current_stream(dev).cuda_stream != (stream or 0):
+        return None
+    return torch.empty(need, dtype=torch.uint8, device="cuda:%d" % dev)
+
+
 def product(A, SA, B, SB, Y, bias=None, work=None, stream=None):
     """Y = A B^T + bias for A (rows x k) and B (columns x k, a weight matrix with a row for each output) in 8-bit form; Y bfloat16 or
-    float16, bias float32.  work: None, or a uint8 tensor of product_work(rows, cols, k) bytes, not used by another call in flight"""
+    float16, bias float32.  work: a uint8 tensor of product_work(rows, cols, k) bytes, not used by another call in flight; None: taken
+    from torch's allocator where there is something to gain and `stream` is torch's current one"""
     types, code, same, dev = _rows(Y, "Y")                     # float32 is refused by the C side
     rows, cols = Y.shape
     k = A.shape[1]
@@ -619,6 +630,8 @@ def product(A, SA, B, SB, Y, bias=None, work=None, stream=None):
     bp, ldb = _rows_arg(B, "B", dev, types.held, cols, k, 16)
     sb, ldsb = _rows_arg(SB, "SB", dev, types.scales, cols, nb, 4)
     yp, ldy = _rows_arg(Y, "Y", dev, same, rows, cols)
+    if work is None and k >= 8192:                             # shorter ones are never split
+        work = _product_room(rows, cols, k, dev, stream)
     wp, wn = (None, 0) if work is None else (_vector_arg(work, "work", dev, types.bytes, work.numel()), work.numel())
     _rows_check(types.lib.speech_rows_product(dev, code, rows, cols, k, ap, lda, sa, ldsa, bp, ldb, sb, ldsb,
                                               None if bias is None else _vector_arg(bias, "bias", dev, (types.f32,), cols), yp, ldy, wp, wn, stream))

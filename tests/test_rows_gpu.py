@@ -449,12 +449,17 @@ def test_product_in_parts(rows, cols, k, dt):
     work = torch.full((need + 64,), 0xA5, dtype=torch.uint8, device="cuda")
     qa, sa, qb, sb, z = _product(rows, cols, k, dt, work[:need])
     assert bool((work[need:] == 0xA5).all()) and not bool((work[:need] == 0xA5).all())
-    whole, short = torch.empty_like(z), torch.empty_like(z)
+    whole, short, own, other = (torch.empty_like(z) for _ in range(4))
     before = work.clone()
-    api.product(qa, sa, qb, sb, whole)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    api.product(qa, sa, qb, sb, whole, work=work[:0])
     api.product(qa, sa, qb, sb, short, work=work[:need - 16])                  # too little: computed whole, nothing left in it
+    api.product(qa, sa, qb, sb, own)                                           # room of its own on torch's current stream, none on another
+    api.product(qa, sa, qb, sb, other, stream=side.cuda_stream)
     torch.cuda.synchronize()
     assert torch.equal(whole, short) and torch.equal(work, before)
+    assert torch.equal(own, z) and torch.equal(other, whole)
 
 
 def _product(rows, cols, k, dt, work=None):
@@ -625,7 +630,7 @@ def test_product_in_parts_in_replayed_graphs():
             if i == 0:
                 api.quantize(X[0], qa, sa, stream=st)
                 api.quantize(X[1], qb, sb, stream=st)
-            api.product(qa, sa, qb, sb, out[i], work=work[i], stream=st)
+            api.product(qa, sa, qb, sb, out[i], work=None if i else work[i], stream=st)   # the second takes its room from the graph's pool
     for _ in range(4):
         X[0].normal_(generator=gen)
         torch.cuda.synchronize()
