@@ -222,7 +222,7 @@ __device__ __forceinline__ void store_e4m3(uint8_t *q, int n, const float (&y)[N
 }
 
 // A row stays in the registers of its TPR threads, CH vectors each, from its one reading to its one writing; the weight's vectors stay
-// there for all of a thread's rows.  Bound by HBM: 31936 x 1024 bf16 with residual and dropout, 262 MB, in 55 us (4.8 TB/s); 7984 x 1024
+// there for all of a thread's rows.  Bound by HBM: 31936 x 1024 bf16 with residual and dropout, 262 MB, in 50 us (5.2 TB/s); 7984 x 1024
 // to 8 bits, 57 MB, in 12.4 us (4.6 TB/s); one row of 2048 in 2.7 us, a launch and two trips to memory.
 template <typename T, int TPR, int CH>
 __global__ __launch_bounds__(TPR > 64 ? TPR : NT) void norm_kernel(const NormParams p)
@@ -388,7 +388,7 @@ __device__ __forceinline__ void grad_store(const NormGradParams &p, size_t row, 
 // As the forward kernel; besides, every thread keeps the sums over its rows of dY h rstd for its columns.  At the end a workgroup
 // adds its row groups' sums in group order and leaves one row of partial sums in `work`: no atomics, the same sums every time.
 // Registers for four waves a SIMD up to 16 values a thread, two above: the grid is sized for that.
-// Bound by HBM: 31936 x 1024 bf16 with residual and dropout, 327 MB, in 71 us (4.6 TB/s), and 5 us for the partial sums.
+// Bound by HBM: 31936 x 1024 bf16 with residual and dropout, 327 MB, in 65 us (5.0 TB/s), and 4.6 us for the partial sums.
 template <typename T, int TPR, int CH>
 __global__ __launch_bounds__(TPR > 64 ? TPR : NT, TPR > NT ? 4 : CH * vec_of<T>() <= 16 ? 4 : 2) void norm_grad_kernel(const NormGradParams p)
 {
