@@ -430,7 +430,8 @@ PRODUCTS = [(1, 1, 1), (1, 16, 128), (1, 512, 2048), (2, 100, 130), (5, 33, 400)
             (1100, 1030, 900), (2048, 2560, 512), (4200, 2100, 300), (2817, 3333, 1152), (33000, 300, 128), (520, 1030, 2064), (300, 1024, 1936), (17, 5000, 1100), (2050, 1000, 1500),
             (4096, 4096, 512), (4300, 3900, 500), (4100, 4000, 1100), (9000, 4200, 640),
             (2000, 1990, 100), (1300, 1100, 1), (1000, 1010, 300), (900, 1024, 384), (4096, 3900, 1040), (3900, 4000, 768), (7900, 4000, 500), (9300, 4200, 640),
-            (98, 2048, 2000), (300, 2048, 500), (500, 600, 1700)]
+            (98, 2048, 2000), (300, 2048, 500), (500, 600, 1700),
+            (1100, 1030, 4500), (2048, 1024, 4224), (1990, 1000, 4097), (1025, 1029, 8191)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
